@@ -588,6 +588,115 @@ ZT_API int zt_linear_xent(const zt_lce_args* args, void* stream);
  * the GEMM expired; its outputs are then incomplete). Synchronises with the device. */
 ZT_API int zt_linear_xent_take_error(int32_t* code);
 
+/* ---- distillation from a teacher's top logits --------------------------------------- */
+
+#define ZT_DISTILL_MAX_TOP 256   /* entries of a row's teacher list */
+
+/* Arguments of zt_distill_rows, zt_distill_rows_backward and zt_distill_rows_grad.
+ *
+ * For a row z of vocab logits, a temperature T and the teacher's list of `top` entries
+ * (i_k, t_k):  q = softmax(z / T),  p = softmax over the list of t_k / T,
+ *   lse  = log sum_v exp(z_v / T)
+ *   loss = T^2 sum_k p_k (log p_k - log q[i_k])
+ *   d loss / dz_v = T (q_v - sum over k with i_k = v of p_k),   d lse / dz_v = q_v / T
+ * in fp32, the gradient rounded once to the logits' dtype. An entry with a negative index
+ * or the logit -inf carries no mass; its other half is not looked at. The same index may
+ * stand several times in a list: its entries' masses add up. A row whose entries all carry
+ * no mass has no teacher: loss, lse and gradient are 0 whatever its logits are. An index
+ * >= vocab, a NaN or +inf among a row's logits or its teacher's, or a row of nothing but
+ * -inf makes that row NaN; a finite mass on a logit of -inf makes its loss +inf. */
+typedef struct zt_distill_args {
+  const void* logits;      /* [rows, vocab] dtype, row stride ld elements, any alignment of its elements */
+  void* grad;              /* [rows, vocab] dtype, row stride ld_grad (backward, grad); may be the logits */
+  const void* top_idx;     /* [rows, top] int32 or int64 token ids */
+  const void* top_logits;  /* [rows, top] the teacher's logits */
+  const float* weight;     /* [rows] gradient of loss (backward; NULL: 0) or the rows' weights (grad) */
+  const float* weight_lse; /* [rows] gradient of lse, or NULL (backward, grad) */
+  float* loss;             /* [rows] out (rows, grad) */
+  float* lse;              /* [rows] out (rows, grad) */
+  float* stats;            /* [rows, 2] out (rows: may be NULL; grad), in (backward): what the backward needs */
+  int64_t rows, vocab, ld, ld_grad;
+  int32_t dtype;           /* ZT_F32, ZT_BF16 or ZT_F16 */
+  int32_t top;             /* 1 .. ZT_DISTILL_MAX_TOP */
+  int32_t idx_bits;        /* 32 or 64 */
+  int32_t top_dtype;       /* ZT_F32, ZT_BF16 or ZT_F16 */
+  float temperature;       /* in [0.001, 1000] */
+  int32_t reserved;
+} zt_distill_args;
+
+/* loss and lse of every row; stats, where given, for a later backward. */
+ZT_API int zt_distill_rows(const zt_distill_args* args, void* stream);
+
+/* grad[r, :] = weight[r] d loss_r / dz_r + weight_lse[r] d lse_r / dz_r from the same
+ * logits, lists and temperature and the stats of zt_distill_rows. */
+ZT_API int zt_distill_rows_backward(const zt_distill_args* args, void* stream);
+
+/* Both at once, for weights known beforehand: loss, lse, stats and
+ * grad[r, :] = weight[r] d loss_r / dz_r (+ weight_lse[r] d lse_r / dz_r). */
+ZT_API int zt_distill_rows_grad(const zt_distill_args* args, void* stream);
+
+/* Arguments of zt_linear_distill. */
+typedef struct zt_linear_distill_args {
+  const void* x;           /* [rows, k] bf16 hidden states, row-major, 16-byte aligned */
+  const void* w;           /* [vocab, k] bf16 lm_head weight, 16-byte aligned */
+  const void* top_idx;     /* as in zt_distill_args */
+  const void* top_logits;
+  float* loss;             /* [rows] out */
+  float* lse;              /* [rows] out */
+  void* workspace;         /* zt_linear_distill_workspace_bytes(rows, vocab, k, top) bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  int64_t rows, vocab, k;  /* k a multiple of 64 */
+  int32_t top, idx_bits, top_dtype;
+  float temperature;
+  int32_t test_stall_loads;  /* test hooks, as in zt_lce_args */
+  int32_t reserved;
+  int64_t test_wait_cycles;
+} zt_linear_distill_args;
+
+/* The lm_head GEMM and zt_distill_rows' loss and lse in one pass, without writing the
+ * logits: z[r, v] = x[r, :] . w[v, :], accumulated in fp32 on the tensor cores and not
+ * rounded. The workspace belongs to one call at a time. Returns the workspace size, 0 on
+ * a bad shape. */
+ZT_API size_t zt_linear_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int32_t top);
+ZT_API int zt_linear_distill(const zt_linear_distill_args* args, void* stream);
+/* The device error flag of the GEMM's bounded waits (0: none); reading clears it. */
+ZT_API int zt_linear_distill_take_error(int32_t* code);
+
+/* ---- query / key norms with the rotary embedding ------------------------------------- */
+
+/* Arguments of zt_qk_norm_rope and zt_qk_norm_rope_backward: q [batch, seq, q_heads,
+ * head_dim] and k [batch, seq, k_heads, head_dim] with element strides over (batch,
+ * position, head) and unit stride inside a head; cos and sin [seq, head_dim], or
+ * [batch * seq, head_dim] with table_batch, contiguous. */
+typedef struct zt_qk_args {
+  const void *q, *k;
+  void *q_out, *k_out;              /* forward: rotated heads (may be q and k themselves, with their strides);
+                                       backward: the gradients of q and k */
+  const void *q_grad, *k_grad;      /* backward: gradients of the rotated heads */
+  const void *q_weight, *k_weight;  /* [head_dim] norm weights */
+  const void *cos, *sin;
+  void *dq_weight, *dk_weight;      /* backward: [head_dim] gradients of the weights, weight_dtype */
+  void* workspace;                  /* backward: zt_qk_norm_rope_workspace_bytes(head_dim) bytes */
+  size_t workspace_bytes;
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3], q_grad_strides[3], k_grad_strides[3];
+  int64_t batch, seq;               /* batch * seq <= 2^25 */
+  int32_t q_heads, k_heads;
+  int32_t head_dim;                 /* even, at most 512 */
+  int32_t dtype;                    /* of the heads and their gradients */
+  int32_t weight_dtype, table_dtype;/* dtype or ZT_F32 */
+  int32_t table_batch;              /* 1: every sequence has its own cos / sin rows */
+  float eps;
+} zt_qk_args;
+
+/* Per head x: n = 1 / sqrt(mean(x^2) + eps), y = w x n, then the rotation of the halves,
+ * out[i] = y[i] cos[i] - y[i + h] sin[i], out[i + h] = y[i + h] cos[i + h] + y[i] sin[i + h]
+ * (h = head_dim / 2), in fp32 with one rounding at the store. What the reference's default
+ * model applies to its queries and keys between projection and attention. */
+ZT_API int zt_qk_norm_rope(const zt_qk_args* args, void* stream);
+/* The gradients of q, k and both weights; cos, sin are constants. Sums in a fixed order. */
+ZT_API int zt_qk_norm_rope_backward(const zt_qk_args* args, void* stream);
+ZT_API size_t zt_qk_norm_rope_workspace_bytes(int32_t head_dim);
+
 /* ---- low-rank directions (distribution "low_rank") on the tensor cores ----------- */
 
 /* Replaces the materialised direction of _sample_z for a 2-D parameter

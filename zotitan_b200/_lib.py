@@ -35,13 +35,17 @@ EXPORTS = ("zt_last_error", "zt_abi_version", "zt_param_key", "zt_philox_words",
            "zt_ipc_export", "zt_ipc_open", "zt_ipc_close", "zt_copy_async",
            "zt_linear_xent_workspace_bytes", "zt_linear_xent", "zt_linear_xent_take_error",
            "zt_gemm_addto", "zt_gemm_take_error",
-           "zt_lowrank_workspace_bytes", "zt_lowrank_prepare", "zt_lowrank_apply", "zt_lowrank_take_error")
+           "zt_lowrank_workspace_bytes", "zt_lowrank_prepare", "zt_lowrank_apply", "zt_lowrank_take_error",
+           "zt_distill_rows", "zt_distill_rows_backward", "zt_distill_rows_grad",
+           "zt_linear_distill_workspace_bytes", "zt_linear_distill", "zt_linear_distill_take_error",
+           "zt_qk_norm_rope", "zt_qk_norm_rope_backward", "zt_qk_norm_rope_workspace_bytes")
 ZT_STATIC_MAX_TENSORS = 1024
 ZT_EGGROLL_MAX_PAIRS = 512
 ZT_EGGROLL_FACTOR_WORK_FLOATS = 64 * 20
 ABI_VERSION = 11
 ZT_LOWRANK_MAX_STREAMS = 128
 ZT_IPC_HANDLE_BYTES = 64
+ZT_DISTILL_MAX_TOP = 256
 
 
 class ZtTensor(ctypes.Structure):
@@ -146,6 +150,39 @@ class ZtLowrankApplyArgs(ctypes.Structure):
                 ("test_wait_cycles", ctypes.c_int64)]
 
 
+class ZtDistillArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("top_idx", ctypes.c_void_p),
+                ("top_logits", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("weight_lse", ctypes.c_void_p),
+                ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("stats", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("ld", ctypes.c_int64),
+                ("ld_grad", ctypes.c_int64), ("dtype", ctypes.c_int32), ("top", ctypes.c_int32),
+                ("idx_bits", ctypes.c_int32), ("top_dtype", ctypes.c_int32), ("temperature", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
+
+
+class ZtLinearDistillArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("top_idx", ctypes.c_void_p),
+                ("top_logits", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("rows", ctypes.c_int64),
+                ("vocab", ctypes.c_int64), ("k", ctypes.c_int64), ("top", ctypes.c_int32), ("idx_bits", ctypes.c_int32),
+                ("top_dtype", ctypes.c_int32), ("temperature", ctypes.c_float), ("test_stall_loads", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("test_wait_cycles", ctypes.c_int64)]
+
+
+class ZtQkArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+                ("q_grad", ctypes.c_void_p), ("k_grad", ctypes.c_void_p), ("q_weight", ctypes.c_void_p),
+                ("k_weight", ctypes.c_void_p), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+                ("dq_weight", ctypes.c_void_p), ("dk_weight", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t), ("q_strides", ctypes.c_int64 * 3),
+                ("k_strides", ctypes.c_int64 * 3), ("q_out_strides", ctypes.c_int64 * 3),
+                ("k_out_strides", ctypes.c_int64 * 3), ("q_grad_strides", ctypes.c_int64 * 3),
+                ("k_grad_strides", ctypes.c_int64 * 3), ("batch", ctypes.c_int64), ("seq", ctypes.c_int64),
+                ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("table_dtype", ctypes.c_int32),
+                ("table_batch", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
 class ZtError(RuntimeError):
     """A C-ABI call returned a nonzero status."""
 
@@ -237,6 +274,22 @@ def load():
     lib.zt_lowrank_apply.argtypes = [ctypes.POINTER(ZtLowrankDesc), ctypes.POINTER(ZtLowrankApplyArgs), P]
     lib.zt_lowrank_take_error.restype = ctypes.c_int
     lib.zt_lowrank_take_error.argtypes = [ctypes.POINTER(ctypes.c_int32)]
+    for name in ("zt_distill_rows", "zt_distill_rows_backward", "zt_distill_rows_grad"):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(ZtDistillArgs), P]
+    lib.zt_linear_distill_workspace_bytes.restype = ctypes.c_size_t
+    lib.zt_linear_distill_workspace_bytes.argtypes = [I64, I64, I64, I32]
+    lib.zt_linear_distill.restype = ctypes.c_int
+    lib.zt_linear_distill.argtypes = [ctypes.POINTER(ZtLinearDistillArgs), P]
+    lib.zt_linear_distill_take_error.restype = ctypes.c_int
+    lib.zt_linear_distill_take_error.argtypes = [ctypes.POINTER(ctypes.c_int32)]
+    for name in ("zt_qk_norm_rope", "zt_qk_norm_rope_backward"):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(ZtQkArgs), P]
+    lib.zt_qk_norm_rope_workspace_bytes.restype = ctypes.c_size_t
+    lib.zt_qk_norm_rope_workspace_bytes.argtypes = [I32]
     lib.zt_plan_workspace_bytes.restype = ctypes.c_size_t
     lib.zt_plan_workspace_bytes.argtypes = [I32]
     if lib.zt_abi_version() != ABI_VERSION:

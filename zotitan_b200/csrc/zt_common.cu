@@ -53,6 +53,15 @@ uint32_t zt_param_key(uint64_t seed, uint32_t n_params, uint32_t index) {
 static_assert(sizeof(zt_pass_cfg) == 240 && offsetof(zt_pass_cfg, zcache) == 128 && offsetof(zt_pass_cfg, zfield_stride) == 144 &&
                   offsetof(zt_pass_cfg, zpush) == 152 && offsetof(zt_pass_cfg, zpush_stride) == 232,
               "zt_pass_cfg layout");
+static_assert(sizeof(zt_distill_args) == 128 && offsetof(zt_distill_args, rows) == 72 &&
+                  offsetof(zt_distill_args, temperature) == 120,
+              "zt_distill_args layout");
+static_assert(sizeof(zt_linear_distill_args) == 120 && offsetof(zt_linear_distill_args, top) == 88 &&
+                  offsetof(zt_linear_distill_args, test_wait_cycles) == 112,
+              "zt_linear_distill_args layout");
+static_assert(sizeof(zt_qk_args) == 304 && offsetof(zt_qk_args, q_strides) == 112 && offsetof(zt_qk_args, batch) == 256 &&
+                  offsetof(zt_qk_args, eps) == 300,
+              "zt_qk_args layout");
 static_assert(sizeof(zt_stream) == 40 && sizeof(zt_tensor) == 64, "zt_stream / zt_tensor layout");
 static_assert(sizeof(zt_lowrank_desc) == 1104 && offsetof(zt_lowrank_desc, p) == 1056 &&
                   offsetof(zt_lowrank_desc, factors_given) == 1096 &&

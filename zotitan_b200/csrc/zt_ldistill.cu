@@ -1,0 +1,495 @@
+// Fused linear distillation: the lm_head GEMM and the loss against a teacher's top logits
+// in one tcgen05 kernel, so no logit reaches HBM.
+//
+//   z[r, v] = X[r, :] . W[v, :]   (fp32 accumulate, not rounded)
+//   lse[r] = log sum_v exp(z[r, v] / T),
+//   loss[r] = T^2 sum_k p_k (log p_k - z[r, i_k] / T + lse[r]),  p = softmax(t_k / T)
+//
+// Bound by the tensor cores where rows are many (2 rows vocab k flops), by reading W where
+// they are few. Three kernels:
+// 1. list_kernel, a warp per row: p from the teacher's list, its entries sorted by token.
+// 2. linear_distill_kernel on CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles, K-block
+//    64, 6 TMA stages, accumulators double-buffered in tensor memory), scheduled like the
+//    cross-entropy GEMM: the vocabulary cut into splits of a few tiles, row blocks fastest,
+//    so that the pairs in flight share W tiles in L2. An epilogue thread owns an accumulator
+//    row; beside the online (max, sum) it follows its row's sorted list through the tiles.
+//    A listed logit is fetched by a one-column load of tensor memory at that column (the
+//    column is the same for the warp's 32 rows, so a warp makes one such load per listed
+//    (row, token) of its rows and tile: about four at 64 entries of 128256 tokens).
+// 3. combine_kernel, a warp per row: the splits' sums in vocabulary order, then the list.
+// Every mbarrier wait is bounded; on expiry the kernel records an error
+// (zt_linear_distill_take_error), drains its own copies and MMAs and frees its tensor memory.
+#include <math.h>
+
+#include "zt_distill.cuh"
+#include "zt_tc.cuh"
+
+namespace {
+
+using namespace zt::tc;
+using namespace zt::distill;
+
+constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA (leader), warps 2-5 epilogue
+constexpr int kStages = 6;
+constexpr uint32_t kHalfRows = 128;
+constexpr uint32_t kStageA = kHalfRows * kBK * 2;  // 16 KB of X
+constexpr uint32_t kStageBytes = 2 * kStageA;       // + 16 KB of W (this CTA's half of the N tile)
+constexpr int kTile = 256;
+constexpr uint32_t kTmemCols = 2 * kTile;
+constexpr size_t kSmem = 1024 + kStages * kStageBytes + 256;
+constexpr uint32_t kIdesc = idesc_bf16(256, 256);
+constexpr int kListWarps = 8;
+enum { kHasTeacher = 0, kNoTeacher = 1, kBadIndex = 2 };
+
+__device__ int g_distill_error = 0;
+
+struct Params {
+  CUtensorMap tmap_x;  // X [rows, k], box {64, 128}
+  CUtensorMap tmap_w;  // W [vocab, k], box {64, 128}
+  TopList list;
+  int32_t* status;     // [rows]
+  int32_t* idx;        // [rows][top] tokens in rising order, INT32_MAX behind the last with mass
+  float* lp;           // [rows][top] log2 p in that order
+  float* z;            // [rows][top] logits in that order
+  float2* partials;    // [n_splits][rows_pad] (m, s)
+  float* loss;
+  float* lse;
+  int32_t rows, vocab, top, k_blocks;
+  int32_t m_tiles, n_tiles, split_tiles, n_splits, rows_pad;
+  float c, temperature;
+  int32_t stall_loads;    // test hook: the loader issues no copies
+  long long wait_cycles;  // bound of every wait
+};
+
+__global__ void __launch_bounds__(32 * kListWarps) list_kernel(const __grid_constant__ Params P) {
+  const int64_t row = (int64_t)blockIdx.x * kListWarps + threadIdx.x / 32;
+  if (row >= P.rows) return;
+  const int lane = threadIdx.x & 31;
+  Teacher t;
+  t.read(P.list, row);
+  t.softmax(P.c);
+  int32_t key[kPer], rank[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    key[e] = t.p[e] != 0.f ? t.idx[e] : INT32_MAX;
+    rank[e] = 0;
+  }
+  // rank of entry (e, lane): entries with a smaller token, or the same and an earlier place
+#pragma unroll
+  for (int o = 0; o < kPer; ++o) {
+    if (32 * o >= P.top) break;
+    for (int l = 0; l < 32; ++l) {
+      const int32_t other = __shfl_sync(0xffffffffu, key[o], l);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (32 * e < P.top) rank[e] += (other < key[e] || (other == key[e] && (o < e || (o == e && l < lane)))) ? 1 : 0;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e)
+    if (lane + 32 * e < P.top) {
+      const int64_t at = row * P.top + rank[e];
+      P.idx[at] = key[e];
+      P.lp[at] = t.lp[e];
+    }
+  if (lane == 0) P.status[row] = !t.any ? kNoTeacher : t.bad ? kBadIndex : kHasTeacher;
+}
+
+__device__ __forceinline__ void item_range(const Params& P, int item, int& mt, int& split, int& nt0, int& nt1) {
+  split = item / P.m_tiles;
+  mt = item - split * P.m_tiles;
+  nt0 = split * P.split_tiles;
+  nt1 = min(nt0 + P.split_tiles, P.n_tiles);
+}
+
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  return __uint_as_float(r);
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    linear_distill_kernel(const __grid_constant__ Params P) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* stage_base = smem;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  uint64_t* full = bars;                    // [kStages], used in the leader
+  uint64_t* empty = bars + kStages;         // [kStages]
+  uint64_t* accf = bars + 2 * kStages;      // [2]
+  uint64_t* acce = bars + 2 * kStages + 2;  // [2], used in the leader
+  uint64_t* drain = bars + 2 * kStages + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&accf[b], 1); mbar_init(&acce[b], 2 * 4); }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {  // warp 0 of both CTAs allocates the pair's tensor memory
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  cluster_sync_all();  // barriers of both CTAs initialised before any cross-CTA signal
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t peer_abort = peer_addr((const void*)abort, rank ^ 1u);
+
+  const int n_items = P.m_tiles * P.n_splits;
+  const int cid = (int)cluster_id_x(), ncl = (int)n_clusters_x();
+  if (warp == 0) {
+    if (lane == 0) {  // ---- TMA producer (both CTAs)
+      int last_phase[kStages];
+      for (int s = 0; s < kStages; ++s) last_phase[s] = -1;
+      uint32_t it = 0;
+      bool ok = !P.stall_loads;
+      for (int item = cid; ok && item < n_items; item += ncl) {
+        int mt, split, nt0, nt1;
+        item_range(P, item, mt, split, nt0, nt1);
+        for (int nt = nt0; ok && nt < nt1; ++nt) {
+          for (int kb = 0; kb < P.k_blocks; ++kb, ++it) {
+            const int s = it % kStages;
+            const uint32_t round = it / kStages;
+            if (!mbar_wait_pair(&empty[s], (round & 1) ^ 1, abort, peer_abort, &g_distill_error, 1, P.wait_cycles)) {
+              ok = false;
+              break;
+            }
+            uint8_t* sa = stage_base + s * kStageBytes;
+            const uint32_t leader_full = peer_addr(&full[s], 0);
+            if (leader) mbar_expect_tx(&full[s], 2 * kStageBytes);
+            tma_load_2d_pair(sa, &P.tmap_x, leader_full, kb * kBK, mt * kTile + (int)rank * (int)kHalfRows);
+            tma_load_2d_pair(sa + kStageA, &P.tmap_w, leader_full, kb * kBK, nt * kTile + (int)rank * (int)kHalfRows);
+            last_phase[s] = (int)(round & 1);
+          }
+        }
+      }
+      // Drain (leader): each armed phase of a full barrier completes only when both CTAs'
+      // copies for it have landed, so no copy is in flight when the pair leaves.
+      if (leader)
+        for (int s = 0; s < kStages; ++s)
+          if (last_phase[s] >= 0) mbar_drain(&full[s], (uint32_t)last_phase[s]);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {  // ---- MMA issuer (leader CTA only)
+      uint32_t it = 0, tcount = 0;
+      bool ok = true, issued = false;
+      for (int item = cid; ok && item < n_items; item += ncl) {
+        int mt, split, nt0, nt1;
+        item_range(P, item, mt, split, nt0, nt1);
+        for (int nt = nt0; ok && nt < nt1; ++nt, ++tcount) {
+          const uint32_t b = tcount & 1;
+          if (!mbar_wait_pair(&acce[b], ((tcount >> 1) & 1) ^ 1, abort, peer_abort, &g_distill_error, 2, P.wait_cycles)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t tmem_d = tmem_base + b * kTile;
+          for (int kb = 0; kb < P.k_blocks; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait_pair(&full[s], (it / kStages) & 1, abort, peer_abort, &g_distill_error, 3, P.wait_cycles)) {
+              ok = false;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t sa = smem_u32(stage_base + s * kStageBytes);
+            const uint32_t sb = sa + kStageA;
+#pragma unroll
+            for (int k = 0; k < kBK / kUmmaK; ++k)
+              umma_bf16_pair<kIdesc>(tmem_d, umma_desc(sa + k * kUmmaK * 2), umma_desc(sb + k * kUmmaK * 2),
+                                     (kb | k) != 0);
+            issued = true;
+            umma_commit_pair(&empty[s]);  // stage s is free in both CTAs once these MMAs have read it
+          }
+          if (!ok) break;
+          umma_commit_pair(&accf[b]);  // accumulator b is complete in both CTAs
+        }
+      }
+      if (issued) {  // wait (bounded) for every MMA issued by this thread before exit
+        umma_commit_pair_local(drain);
+        mbar_drain(drain, 0);
+      }
+    }
+  } else {  // ---- epilogue: warps 2..5 of both CTAs; each thread owns one accumulator row
+    const int q = warp & 3;
+    const int row_local = q * 32 + lane;
+    const uint32_t leader_acce0 = peer_addr(&acce[0], 0), leader_acce1 = peer_addr(&acce[1], 0);
+    uint32_t tcount = 0;
+    bool ok = true;
+    for (int item = cid; ok && item < n_items; item += ncl) {
+      int mt, split, nt0, nt1;
+      item_range(P, item, mt, split, nt0, nt1);
+      const int row = mt * kTile + (int)rank * (int)kHalfRows + row_local;
+      // the row's list from this split's first column on: its place, its next two tokens
+      const int32_t* list = P.idx + (int64_t)row * P.top;
+      int pos = P.top, next = INT32_MAX, after = INT32_MAX;
+      if (row < P.rows) {
+        int lo = 0, hi = P.top;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (list[mid] < nt0 * kTile) lo = mid + 1;
+          else hi = mid;
+        }
+        pos = lo;
+        if (pos < P.top) next = list[pos];
+        if (pos + 1 < P.top) after = list[pos + 1];
+      }
+      Stat st{-INFINITY, 0.f};
+      for (int nt = nt0; nt < nt1; ++nt, ++tcount) {
+        const uint32_t b = tcount & 1;
+        int okw = 1;
+        if (lane == 0) okw = mbar_wait_pair(&accf[b], (tcount >> 1) & 1, abort, peer_abort, &g_distill_error, 4, P.wait_cycles) ? 1 : 0;
+        okw = __shfl_sync(0xffffffffu, okw, 0);
+        if (!okw) { ok = false; break; }
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + b * kTile;
+        const int tile0 = nt * kTile;
+        for (;;) {  // the listed columns of this tile, one column of the warp's rows at a time
+          const unsigned has = __ballot_sync(0xffffffffu, next < tile0 + kTile);
+          if (!has) break;
+          const int col = __shfl_sync(0xffffffffu, next, __ffs(has) - 1);
+          const float v = tmem_ld1(acc + (uint32_t)(col - tile0));
+          if (next == col) {
+            P.z[(int64_t)row * P.top + pos] = v;
+            ++pos;
+            next = after;
+            after = pos + 1 < P.top ? list[pos + 1] : INT32_MAX;
+          }
+          __syncwarp();
+        }
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld32(acc + (uint32_t)c0, r);
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          if (tile0 + c0 + 32 > P.vocab) {  // the padded columns of the last tile
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (tile0 + c0 + j >= P.vocab) v[j] = -INFINITY;
+          }
+          absorb(st, v, P.c);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(b ? leader_acce1 : leader_acce0);  // accumulator b may be overwritten
+      }
+      if (ok && row < P.rows) P.partials[(size_t)split * P.rows_pad + row] = make_float2(st.m, st.s);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while its peer may still signal it or read its shared memory
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 0) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+}
+
+__global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_constant__ Params P) {
+  const int64_t row = (int64_t)blockIdx.x * kListWarps + threadIdx.x / 32;
+  if (row >= P.rows) return;
+  const int lane = threadIdx.x & 31;
+  Stat st{-INFINITY, 0.f};
+  for (int sp = lane; sp < P.n_splits; sp += 32) {
+    const float2 o = P.partials[(size_t)sp * P.rows_pad + row];
+    st = merge(st, Stat{o.x, o.y}, P.c);
+  }
+  st = warp_merge(st, P.c);
+  if (st.m == -INFINITY) st.s = NAN;
+  const float ls = log2f(st.s);
+  float a = 0.f;
+  for (int k = lane; k < P.top; k += 32) {
+    const int64_t at = row * P.top + k;
+    if (P.idx[at] != INT32_MAX) a = fmaf(exp2f(P.lp[at]), P.lp[at] - ((P.z[at] - st.m) * P.c - ls), a);
+  }
+  a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
+  if (lane == 0) {
+    const int32_t status = P.status[row];
+    P.loss[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : a;
+    P.lse[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : st.m / P.temperature + logf(st.s);
+  }
+}
+
+// Per-device kernel attributes and the number of CTA pairs resident at once.
+int g_max_pairs[64] = {0};
+
+int prepare(int dev) {
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if (g_max_pairs[dev] > 0) return ZT_OK;
+  if (int rc = zt::check_cuda(cudaFuncSetAttribute(linear_distill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)kSmem), "zt_linear_distill: shared memory attribute"))
+    return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)(zt::sm_count() / 2));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  int n = 0;
+  if (int rc = zt::check_cuda(cudaOccupancyMaxActiveClusters(&n, linear_distill_kernel, &cfg),
+                              "zt_linear_distill: cudaOccupancyMaxActiveClusters"))
+    return rc;
+  if (n <= 0) return zt::set_error(ZT_ERR_CUDA, "zt_linear_distill: no CTA pair fits on this GPU");
+  g_max_pairs[dev] = n;
+  return ZT_OK;
+}
+
+// Vocabulary split: the split length (in 256-column tiles) whose round-robin schedule over
+// `pairs` CTA pairs has the smallest longest queue, preferring longer splits on ties.
+struct Split {
+  int32_t m_tiles, n_tiles, split_tiles, n_splits, rows_pad;
+};
+
+Split choose_split(int64_t rows, int64_t vocab, int pairs) {
+  Split sp;
+  sp.m_tiles = (int32_t)((rows + kTile - 1) / kTile);
+  sp.n_tiles = (int32_t)((vocab + kTile - 1) / kTile);
+  sp.rows_pad = sp.m_tiles * kTile;
+  long long best = -1;
+  sp.split_tiles = sp.n_tiles;
+  for (int st = 1; st <= sp.n_tiles && st <= 64; ++st) {
+    const long long splits = (sp.n_tiles + st - 1) / st;
+    const long long items = splits * sp.m_tiles;
+    const long long queue = (items + pairs - 1) / pairs * st;
+    if (best < 0 || queue <= best) {
+      best = queue;
+      sp.split_tiles = st;
+    }
+  }
+  sp.n_splits = (sp.n_tiles + sp.split_tiles - 1) / sp.split_tiles;
+  return sp;
+}
+
+int device_pairs(int* dev, int* pairs) {
+  if (int rc = zt::check_cuda(cudaGetDevice(dev), "zt_linear_distill: cudaGetDevice")) return rc;
+  if (*dev < 0 || *dev >= 64) return zt::set_error(ZT_ERR_LIMIT, "zt_linear_distill: device ordinal >= 64");
+  if (int rc = prepare(*dev)) return rc;
+  *pairs = g_max_pairs[*dev];
+  return ZT_OK;
+}
+
+// The items (row blocks x splits, at most one split per tile) are counted in 32 bits.
+int check_shape(int64_t rows, int64_t vocab, int64_t k, int32_t top) {
+  if (rows <= 0 || rows > (int64_t)1 << 28) return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: rows outside [1, 2^28]");
+  if (vocab <= 0 || vocab > (int64_t)1 << 28) return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: vocab outside [1, 2^28]");
+  if (k <= 0 || k % kBK != 0 || k > (int64_t)1 << 30)
+    return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: k must be a positive multiple of 64");
+  if (top < 1 || top > kMaxTop)
+    return zt::set_error(ZT_ERR_LIMIT, "zt_linear_distill: the teacher's list must have 1 to 256 entries");
+  if (((rows + kTile - 1) / kTile) * ((vocab + kTile - 1) / kTile) > (int64_t)INT32_MAX / 2)
+    return zt::set_error(ZT_ERR_LIMIT, "zt_linear_distill: rows x vocab above 2^46");
+  return ZT_OK;
+}
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// The workspace: partials, sorted tokens, log2 p, logits, status.
+struct Layout {
+  size_t idx, lp, z, status, total;
+};
+
+Layout layout(const Split& sp, int64_t rows, int32_t top) {
+  const size_t entries = up256((size_t)rows * (size_t)top * 4);
+  Layout L;
+  L.idx = up256(sizeof(float2) * (size_t)sp.n_splits * (size_t)sp.rows_pad);
+  L.lp = L.idx + entries;
+  L.z = L.lp + entries;
+  L.status = L.z + entries;
+  L.total = L.status + up256((size_t)rows * 4);
+  return L;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t zt_linear_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int32_t top) {
+  zt::clear_error();
+  if (check_shape(rows, vocab, k, top)) return 0;
+  int dev = 0, pairs = 0;
+  if (device_pairs(&dev, &pairs)) return 0;
+  return layout(choose_split(rows, vocab, pairs), rows, top).total;
+}
+
+int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
+  zt::clear_error();
+  if (!a || !a->x || !a->w || !a->loss || !a->lse || !a->workspace)
+    return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: null pointer");
+  if (int rc = check_shape(a->rows, a->vocab, a->k, a->top)) return rc;
+  if (int rc = check_list(a->top_idx, a->top_logits, a->top, a->idx_bits, a->top_dtype, a->temperature, false,
+                          "zt_linear_distill"))
+    return rc;
+  auto mis16 = [](const void* p) { return ((uintptr_t)p & 15u) != 0; };
+  if (mis16(a->x) || mis16(a->w) || mis16(a->workspace))
+    return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: x, w and workspace must be 16-byte aligned");
+  int dev = 0, pairs = 0;
+  if (int rc = device_pairs(&dev, &pairs)) return rc;
+  const Split sp = choose_split(a->rows, a->vocab, pairs);
+  const Layout L = layout(sp, a->rows, a->top);
+  if (a->workspace_bytes < L.total) return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: workspace too small");
+  EncodeFn enc = nullptr;
+  if (int rc = get_encode(&enc, "zt_linear_distill")) return rc;
+  Params P;
+  if (int rc = make_map_bf16(enc, &P.tmap_x, a->x, (uint64_t)a->rows, (uint64_t)a->k, kHalfRows, "zt_linear_distill"))
+    return rc;
+  if (int rc = make_map_bf16(enc, &P.tmap_w, a->w, (uint64_t)a->vocab, (uint64_t)a->k, kHalfRows, "zt_linear_distill"))
+    return rc;
+  char* ws = static_cast<char*>(a->workspace);
+  P.list = TopList{a->top_idx, a->top_logits, a->top, a->idx_bits == 64, a->top_dtype, a->vocab};
+  P.partials = reinterpret_cast<float2*>(ws);
+  P.idx = reinterpret_cast<int32_t*>(ws + L.idx);
+  P.lp = reinterpret_cast<float*>(ws + L.lp);
+  P.z = reinterpret_cast<float*>(ws + L.z);
+  P.status = reinterpret_cast<int32_t*>(ws + L.status);
+  P.loss = a->loss;
+  P.lse = a->lse;
+  P.rows = (int32_t)a->rows;
+  P.vocab = (int32_t)a->vocab;
+  P.top = a->top;
+  P.k_blocks = (int32_t)(a->k / kBK);
+  P.m_tiles = sp.m_tiles;
+  P.n_tiles = sp.n_tiles;
+  P.split_tiles = sp.split_tiles;
+  P.n_splits = sp.n_splits;
+  P.rows_pad = sp.rows_pad;
+  P.c = kLog2e / a->temperature;
+  P.temperature = a->temperature;
+  P.stall_loads = a->test_stall_loads ? 1 : 0;
+  P.wait_cycles = a->test_wait_cycles > 0 ? (long long)a->test_wait_cycles : kWaitCycles;
+  const int items = sp.m_tiles * sp.n_splits;
+  const int clusters = items < pairs ? items : pairs;
+  cudaStream_t s = zt::as_stream(stream);
+  const unsigned row_blocks = (unsigned)((a->rows + kListWarps - 1) / kListWarps);
+  list_kernel<<<row_blocks, 32 * kListWarps, 0, s>>>(P);
+  if (int rc = zt::check_cuda(cudaGetLastError(), "zt_linear_distill: list launch")) return rc;
+  linear_distill_kernel<<<2 * clusters, kThreads, kSmem, s>>>(P);
+  if (int rc = zt::check_cuda(cudaGetLastError(), "zt_linear_distill: gemm launch")) return rc;
+  combine_kernel<<<row_blocks, 32 * kListWarps, 0, s>>>(P);
+  return zt::check_cuda(cudaGetLastError(), "zt_linear_distill: combine launch");
+}
+
+int zt_linear_distill_take_error(int32_t* code) {
+  zt::clear_error();
+  if (!code) return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill_take_error: null pointer");
+  int v = 0;
+  if (int rc = zt::check_cuda(cudaMemcpyFromSymbol(&v, g_distill_error, sizeof(int)), "zt_linear_distill_take_error: read"))
+    return rc;
+  const int zero = 0;
+  if (int rc = zt::check_cuda(cudaMemcpyToSymbol(g_distill_error, &zero, sizeof(int)), "zt_linear_distill_take_error: clear"))
+    return rc;
+  *code = v;
+  return ZT_OK;
+}
+
+}  // extern "C"

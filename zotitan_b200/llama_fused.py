@@ -19,7 +19,17 @@ LlamaMLP instance of a model for one that calls this package's kernels:
   (LoRA wrappers, ragged rows) the projections as modules and `zt_eggroll_swiglu`
   (bf16(bf16(silu(g)) * u), torch's rounding points). Then the down projection.
 
-Each fused forward defers to the module's own forward when gradients are enabled,
+Decoders whose attention norms every query and key head before the rotation
+(transformers' Qwen3, the reference's default model, zotitan/model.py) take the same
+RMSNorm and MLP and an attention of their own:
+
+- attention with head norms: both norms and the rotary embedding in one pass over the
+  projection outputs, in place (`zt_qk_norm_rope`; fp32 inside, rounded once where the
+  modules round after the norm, its weight, each rotary product and their sum). With
+  gradients enabled the same kernel runs out of place and brings its backward
+  (`kernels.qk_norm_rope`), in bf16, fp16 or fp32.
+
+Each other fused forward defers to the module's own forward when gradients are enabled,
 the activations are not bf16 on a CUDA device, the layout does not fit (head_dim not a
 multiple of 16, per-sequence position ids), or the MLP's activation is not SiLU.
 `unfuse_llama(model)` restores the original forwards.
@@ -93,6 +103,38 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
     return self.o_proj(out.reshape(bsz, T, -1).contiguous()), weights
 
 
+def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None,
+                               **kwargs):
+    cos, sin = position_embeddings if position_embeddings is not None else (None, None)
+    hd = self.head_dim
+    wq, wk = self.q_norm.weight, self.k_norm.weight
+    eps = self.q_norm.variance_epsilon
+    dt = hidden_states.dtype
+    if (not hidden_states.is_cuda or dt not in (torch.bfloat16, torch.float16, torch.float32) or cos is None
+            or hidden_states.dim() != 3 or hidden_states.numel() == 0 or cos.dim() != 3
+            or cos.shape[0] not in (1, hidden_states.shape[0]) or cos.shape[1:] != (hidden_states.shape[1], hd) or hd % 2
+            or hd > 512 or eps != self.k_norm.variance_epsilon or wq.shape != (hd,) or wk.shape != (hd,)
+            or wq.dtype != wk.dtype or wq.dtype not in (dt, torch.float32) or cos.dtype not in (dt, torch.float32)
+            or torch.is_autocast_enabled("cuda")):
+        return self._zt_orig_forward(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
+    from transformers.models.qwen3.modeling_qwen3 import ALL_ATTENTION_FUNCTIONS, eager_attention_forward
+    bsz, T, _ = hidden_states.shape
+    q = self.q_proj(hidden_states).view(bsz, T, -1, hd)
+    k = self.k_proj(hidden_states).view(bsz, T, -1, hd)
+    v = self.v_proj(hidden_states).view(bsz, T, -1, hd).transpose(1, 2)
+    norm = K.qk_norm_rope if torch.is_grad_enabled() else K.qk_norm_rope_
+    q, k = norm(q, k, wq, wk, cos, sin, eps)
+    q, k = q.transpose(1, 2), k.transpose(1, 2)
+    if past_key_values is not None:
+        k, v = past_key_values.update(k, v, self.layer_idx)
+    if _ASSUME_CAUSAL and past_key_values is None and self.sliding_window is None:
+        attention_mask = None   # purely causal: SDPA's is_causal (see assume_causal)
+    attn = ALL_ATTENTION_FUNCTIONS.get_interface(self.config._attn_implementation, eager_attention_forward)
+    out, weights = attn(self, q, k, v, attention_mask, dropout=0.0 if not self.training else self.attention_dropout,
+                        scaling=self.scaling, sliding_window=self.sliding_window, **kwargs)
+    return self.o_proj(out.reshape(bsz, T, -1).contiguous()), weights
+
+
 def is_silu(act) -> bool:
     """torch's SiLU module or transformers' SiLUActivation (both F.silu)."""
     return isinstance(act, nn.SiLU) or type(act).__name__ == "SiLUActivation"
@@ -125,11 +167,12 @@ def _mlp_forward(self, x):
     return self.down_proj(K.eggroll_swiglu(g, u))
 
 
-_FORWARDS = {"LlamaRMSNorm": _rmsnorm_forward, "LlamaAttention": _attention_forward, "LlamaMLP": _mlp_forward}
+_FORWARDS = {"LlamaRMSNorm": _rmsnorm_forward, "LlamaAttention": _attention_forward, "LlamaMLP": _mlp_forward,
+             "Qwen3RMSNorm": _rmsnorm_forward, "Qwen3Attention": _qk_norm_attention_forward, "Qwen3MLP": _mlp_forward}
 
 
 def fuse_llama(model: nn.Module) -> int:
-    """Install the fused forwards on every Llama RMSNorm / attention / MLP module of
+    """Install the fused forwards on every Llama or Qwen3 RMSNorm / attention / MLP module of
     `model`; returns how many modules were changed. Idempotent."""
     n = 0
     for m in model.modules():

@@ -10,6 +10,12 @@ that is not a multiple of 64) go through the lm_head GEMM in row chunks and
 the reference's torch path (zotitan/losses.py:55-79), run eagerly. Both return
 (ce, z_loss | None, extra | None) with ce and z_loss kept apart, as the reference's
 contract does.
+
+``distill_xentropy`` scores against a teacher instead of labels: each position's loss is the
+divergence from the teacher's top logits there (``head_distill``). Without gradients, as the
+zeroth-order losses run, the head's GEMM and the loss are one kernel (``zt_linear_distill``);
+with gradients and a frozen head the logits exist one chunk of rows at a time and become their
+own gradient in place (``zt_distill_rows_grad``).
 """
 from __future__ import annotations
 
@@ -100,6 +106,86 @@ def fused_xentropy(model, batch, z_loss_weight: float, compute_accuracy: bool):
         return ce, None, extra
     z_loss = z_loss_weight * (lse.square() * mask).sum() / n
     return ce, z_loss, extra
+
+
+class _FrozenHeadDistill(torch.autograd.Function):
+    """head_distill through a head that is not trained: a chunk's logits turn into
+    dloss_r/dlogits_r in place and then into dloss_r/dhidden_r, which the backward scales by
+    each row's upstream gradient. lse is not differentiable here."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, top_idx, top_logits, temperature, chunk_rows):
+        R, dev = hidden.shape[0], hidden.device
+        loss = torch.empty(R, dtype=torch.float32, device=dev)
+        lse = torch.empty(R, dtype=torch.float32, device=dev)
+        dx = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev)
+        ones = torch.ones(min(R, chunk_rows), dtype=torch.float32, device=dev)
+        for r0 in range(0, R, chunk_rows):
+            r1 = min(R, r0 + chunk_rows)
+            logits = F.linear(hidden[r0:r1], weight, bias)
+            loss[r0:r1], lse[r0:r1], grad = K.distill_rows_grad(logits, top_idx[r0:r1], top_logits[r0:r1], ones[:r1 - r0],
+                                                                temperature, out=logits)
+            torch.mm(grad, weight, out=dx[r0:r1])
+            del logits, grad
+        ctx.save_for_backward(dx)
+        ctx.mark_non_differentiable(lse)
+        return loss, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _):
+        dx, = ctx.saved_tensors
+        return (dx * g[:, None]).to(dx.dtype), None, None, None, None, None, None
+
+
+def head_distill(hidden: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.Tensor, weight: torch.Tensor, bias=None,
+                 temperature: float = 1.0, chunk_rows: int = CHUNK_ROWS):
+    """Per-row (loss, lse) of hidden rows [R, d] through the head against the teacher's lists
+    [R, top] (kernels.distill_rows): without gradients the fused kernel (zt_linear_distill)
+    when it takes the operands, which does not round the logits, else a chunk of rows at a
+    time through the GEMM and zt_distill_rows. Differentiable in hidden, and in the head
+    where that requires grad (then the whole logits are kept, as the backward needs them);
+    lse is differentiable only in that last form."""
+    train_head = weight.requires_grad or (bias is not None and bias.requires_grad)
+    if torch.is_grad_enabled() and train_head:
+        return K.distill_rows(F.linear(hidden, weight, bias), top_idx, top_logits, temperature)
+    if torch.is_grad_enabled() and hidden.requires_grad:
+        return _FrozenHeadDistill.apply(hidden, weight, bias, top_idx, top_logits, temperature, chunk_rows)
+    if bias is None and K.linear_xent_supported(hidden, weight):
+        return K.linear_distill(hidden, weight, top_idx, top_logits, temperature)
+    R, dev = hidden.shape[0], hidden.device
+    loss = torch.empty(R, dtype=torch.float32, device=dev)
+    lse = torch.empty(R, dtype=torch.float32, device=dev)
+    for r0 in range(0, R, chunk_rows):
+        r1 = min(R, r0 + chunk_rows)
+        logits = F.linear(hidden[r0:r1], weight, bias)
+        loss[r0:r1], lse[r0:r1] = K.distill_rows(logits, top_idx[r0:r1], top_logits[r0:r1], temperature)
+        del logits
+    return loss, lse
+
+
+def distill_xentropy(model, batch, temperature: float = 1.0, z_loss_weight: float = 0.0):
+    """The distillation scorer: decoder forward, then head_distill of every position against
+    batch["teacher_idx"], batch["teacher_logits"] [B, S, top] (the teacher's logits for the
+    token after position s; index -1 or logit -inf: no entry). Positions without an entry
+    (padding, the last one of a sequence) do not count. Returns (loss, z_loss | None, None)
+    as the cross-entropy scorers do: loss = mean over the counted positions,
+    z_loss = z_loss_weight * mean(lse^2) with lse = logsumexp(logits / temperature)."""
+    m = getattr(model, "_orig_mod", model)
+    hidden = m.get_decoder()(input_ids=batch["input_ids"], attention_mask=batch.get("attention_mask"),
+                             use_cache=False).last_hidden_state
+    head = m.get_output_embeddings()
+    idx, val = batch["teacher_idx"], batch["teacher_logits"]
+    if idx.dim() != 3 or idx.shape[:2] != hidden.shape[:2] or val.shape != idx.shape:
+        raise ValueError("teacher_idx and teacher_logits must be [batch, positions, top]")
+    hidden = hidden.reshape(-1, hidden.shape[-1])
+    idx, val = idx.reshape(-1, idx.shape[-1]), val.reshape(-1, val.shape[-1])
+    if z_loss_weight != 0.0 and torch.is_grad_enabled() and hidden.requires_grad and not head.weight.requires_grad:
+        raise NotImplementedError("the z-loss has no gradient through a frozen head: use z_loss_weight=0")
+    loss, lse = head_distill(hidden, idx, val, head.weight, getattr(head, "bias", None), temperature)
+    n = ((idx >= 0) & (val != -float("inf"))).any(-1).sum().clamp_min(1)
+    value = loss.sum() / n
+    return value, None if z_loss_weight == 0.0 else z_loss_weight * lse.square().sum() / n, None
 
 
 def get_xentropy(fused: bool, compile_mode: str | None = None):

@@ -16,7 +16,7 @@ from typing import Iterator, Protocol
 import torch
 
 from .data import synthetic_token_batches
-from .losses import get_xentropy, torch_xentropy  # noqa: F401  (torch_xentropy re-exported)
+from .losses import distill_xentropy, get_xentropy, torch_xentropy  # noqa: F401  (torch_xentropy re-exported)
 
 Metric = torch.Tensor | float
 
@@ -74,6 +74,26 @@ class CrossEntropyCriterion:
         if extra:
             metrics.update(extra)
         return value, metrics
+
+
+class DistillationCriterion:
+    """value = distill + z_loss; metrics {"distill", "z_loss"}: the divergence from a
+    teacher's top logits (losses.distill_xentropy) on batches that carry teacher_idx and
+    teacher_logits [B, S, top]. A criterion as CrossEntropyCriterion is, so a RubricObjective
+    can weigh both."""
+    name = "distill"
+    differentiable = True
+
+    def __init__(self, temperature: float = 1.0, z_loss_weight: float = 0.0):
+        self.temperature = temperature
+        self.z_loss_weight = z_loss_weight
+
+    def __call__(self, model, batch):
+        loss, z_loss, _ = distill_xentropy(model, batch, self.temperature, self.z_loss_weight)
+        metrics: dict[str, Metric] = {"distill": loss}
+        if z_loss is not None:
+            metrics["z_loss"] = z_loss
+        return (loss if z_loss is None else loss + z_loss), metrics
 
 
 class RubricObjective:
