@@ -277,17 +277,17 @@ def load():
     for name in ("zt_distill_rows", "zt_distill_rows_backward", "zt_distill_rows_grad"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
-        fn.argtypes = [ctypes.POINTER(ZtDistillArgs), P]
+        fn.argtypes = [P, P]   # a ZtDistillArgs, by reference or as packed bytes
     lib.zt_linear_distill_workspace_bytes.restype = ctypes.c_size_t
     lib.zt_linear_distill_workspace_bytes.argtypes = [I64, I64, I64, I32]
     lib.zt_linear_distill.restype = ctypes.c_int
-    lib.zt_linear_distill.argtypes = [ctypes.POINTER(ZtLinearDistillArgs), P]
+    lib.zt_linear_distill.argtypes = [P, P]
     lib.zt_linear_distill_take_error.restype = ctypes.c_int
     lib.zt_linear_distill_take_error.argtypes = [ctypes.POINTER(ctypes.c_int32)]
     for name in ("zt_qk_norm_rope", "zt_qk_norm_rope_backward"):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
-        fn.argtypes = [ctypes.POINTER(ZtQkArgs), P]
+        fn.argtypes = [P, P]
     lib.zt_qk_norm_rope_workspace_bytes.restype = ctypes.c_size_t
     lib.zt_qk_norm_rope_workspace_bytes.argtypes = [I32]
     lib.zt_plan_workspace_bytes.restype = ctypes.c_size_t

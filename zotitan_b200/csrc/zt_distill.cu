@@ -164,12 +164,23 @@ __device__ __forceinline__ Stat final_stat(Stat st, bool bad) {
   return st;
 }
 
+// The row's logits at the list's indices inside [lo, hi).
+template <int DT>
+__device__ __forceinline__ void gather(List& s, const typename El<DT>::T* row, int top, int32_t lo, int32_t hi) {
+#pragma unroll 4
+  for (int k = threadIdx.x & 31; k < top; k += 32) {
+    const int32_t i = s.idx[k];
+    s.z[k] = i >= lo && i < hi ? El<DT>::to(row[i]) : 0.f;
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
   constexpr int V = El<DT>::kVec, U = 4;
   __shared__ Stat red[kWarps];
   __shared__ Stat mine;
+  __shared__ List list;
   __shared__ int none;   // this row has no teacher: its logits need not be read
   const int parts = P.parts;
   const int64_t row = blockIdx.x / parts;
@@ -179,14 +190,13 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const __grid_
   __syncthreads();
 
   Teacher t;
-  float zk[kPer];
   if (tid >= kStream) {
-    t.read(P.list, row);
+    t = read_list(list, P.list, row);
     if (!t.any && (tid & 31) == 0) *(volatile int*)&none = 1;
-    const T* z = static_cast<const T*>(P.z) + row * P.ld;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) zk[e] = part == 0 && t.idx[e] >= 0 ? El<DT>::to(z[t.idx[e]]) : 0.f;
-    t.softmax(P.c);
+    if (part == 0) {
+      gather<DT>(list, static_cast<const T*>(P.z) + row * P.ld, P.list.top, 0, P.vocab);
+      list_softmax(list, P.list.top, P.c);
+    }
   } else {
     const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
     Stat st{-INFINITY, 0.f};
@@ -231,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const __grid_
   }
   if (tid >= kStream && part == 0) {
     st = final_stat(st, t.bad);
-    const float loss = list_loss(t, zk, st, P.c, P.temperature);
+    const float loss = list_loss(list, P.list.top, st, P.c, P.temperature);
     if ((tid & 31) == 0) {
       if (!t.any) st.s = 0.f;
       P.loss[row] = t.any ? (t.bad ? NAN : loss) : 0.f;
@@ -242,38 +252,28 @@ __global__ void __launch_bounds__(kThreads) distill_forward_kernel(const __grid_
   if (parts > 1) cluster_sync_all();   // no CTA leaves while its sum may still be read
 }
 
-// The gradient at the listed indices, T-scaled and complete: A q - B (sum of p over the
-// entries with this index), written over the dense part's value there. Entries that share
-// an index write the same value.
-template <int DT> struct Patch {
-  float v[kPer];
+// The gradient at the listed indices is A q - B (the sum of p over the entries with that
+// index): list_sums leaves that sum, in list order, in lp, and patch writes the gradient over
+// the dense part's value there. Entries that share an index write the same value.
+__device__ __forceinline__ void list_sums(List& s, int top) {
+  __syncwarp();
+  for (int k = threadIdx.x & 31; k < top; k += 32) {
+    const int32_t own = s.idx[k];
+    float a = 0.f;
+#pragma unroll 8
+    for (int j = 0; j < top; ++j) a += s.idx[j] == own ? s.p[j] : 0.f;
+    s.lp[k] = a;
+  }
+}
 
-  __device__ __forceinline__ void make(const Teacher& t, const float (&zk)[kPer], const Stat& st, float A, float B, float c,
-                                       int32_t top) {
-    float p[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) p[e] = 0.f;
-    // sum of p over equal indices, in list order
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      if (32 * e >= top) break;
-      for (int l = 0; l < 32; ++l) {
-        const int32_t oi = __shfl_sync(0xffffffffu, t.idx[e], l);
-        const float op = __shfl_sync(0xffffffffu, t.p[e], l);
-#pragma unroll
-        for (int f = 0; f < kPer; ++f)
-          if (32 * f < top && oi == t.idx[f]) p[f] += op;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = A * (ex2((zk[e] - st.m) * c) / st.s) - B * p[e];
+template <int DT>
+__device__ __forceinline__ void patch(const List& s, int top, const Stat& st, float A, float B, float c,
+                                      typename El<DT>::T* grad, int32_t lo, int32_t hi) {
+  for (int k = threadIdx.x & 31; k < top; k += 32) {
+    const int32_t i = s.idx[k];
+    if (i >= lo && i < hi) grad[i] = El<DT>::from(A * (ex2((s.z[k] - st.m) * c) / st.s) - B * s.lp[k]);
   }
-  __device__ __forceinline__ void store(const Teacher& t, typename El<DT>::T* grad, int32_t lo, int32_t hi) const {
-#pragma unroll
-    for (int e = 0; e < kPer; ++e)
-      if (t.idx[e] >= lo && t.idx[e] < hi) grad[t.idx[e]] = El<DT>::from(v[e]);
-  }
-};
+}
 
 // dz = a 2^((z - m) c) over a span; the gradient's row has its own 16-byte phase.
 template <int DT> __device__ __forceinline__ float dense(float z, float m, float a, float c) { return a * ex2((z - m) * c); }
@@ -282,8 +282,10 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
   constexpr int V = El<DT>::kVec, U = 4;
-  const int64_t row = blockIdx.x / P.parts;
-  const int part = (int)(blockIdx.x - row * P.parts);
+  // last rows first: those the forward read last may still be in L2
+  const unsigned place = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = place / P.parts;
+  const int part = (int)(place - row * P.parts);
   const int tid = threadIdx.x;
   const float2 s2 = P.stats[row];
   const Stat st{s2.x, s2.y};
@@ -294,15 +296,12 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const __grid
   const float B = g * P.temperature, A = B + gl / P.temperature;
   const bool in_place = P.grad == P.z;
 
-  Teacher t;
-  Patch<DT> patch;
+  __shared__ List list;
   if (tid >= kStream && !none) {
-    t.read(P.list, row);
-    float zk[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) zk[e] = t.idx[e] >= sp.lo && t.idx[e] < sp.hi ? El<DT>::to(sp.row[t.idx[e]]) : 0.f;
-    t.softmax(P.c);
-    patch.make(t, zk, st, A, B, P.c, P.list.top);
+    read_list(list, P.list, row);
+    gather<DT>(list, sp.row, P.list.top, sp.lo, sp.hi);
+    list_softmax(list, P.list.top, P.c);
+    list_sums(list, P.list.top);
   }
   if (in_place) __syncthreads();   // the listed logits are read before they are overwritten
   if (tid < kStream) {
@@ -342,7 +341,142 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const __grid
     }
   }
   __syncthreads();
-  if (tid >= kStream && !none) patch.store(t, out, sp.lo, sp.hi);
+  if (tid >= kStream && !none) patch<DT>(list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
+}
+
+// Loss and gradient at once: a cluster's CTAs hold the row, so it is read once. A thread
+// copies its own vectors to shared memory (cp.async: no registers, no barrier), adds them up
+// as they land, and after the cluster has merged its sums turns the same vectors into the
+// gradient.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(zt::tc::smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) distill_grad_kernel(const __grid_constant__ RowsParams P) {
+  using T = typename El<DT>::T;
+  constexpr int V = El<DT>::kVec, U = 2, D = 8;   // D groups of U vectors a thread in flight
+  extern __shared__ uint4 held[];
+  __shared__ Stat red[kWarps];
+  __shared__ Stat mine;
+  __shared__ List list;
+  __shared__ int none, bad;   // no teacher; an index that does not exist
+  const int parts = P.parts;
+  const int64_t row = blockIdx.x / parts;
+  const int part = (int)(blockIdx.x - row * parts);
+  const int tid = threadIdx.x;
+  const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
+  const uint4* v = sp.vec();
+  if (tid < kStream) {   // the first groups are on their way before anything else
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = tid + (d * U + j) * kStream;
+        if (i < sp.n_vec) copy16(held + i, v + i);
+      }
+      copy_commit();
+    }
+  }
+  if (tid == 0) none = 0;
+  __syncthreads();
+
+  float head = 0.f, tail = 0.f;   // the elements before and behind the vectors
+  if (tid >= kStream) {
+    const Teacher t = read_list(list, P.list, row);
+    if ((tid & 31) == 0) {
+      bad = t.bad;
+      if (!t.any) *(volatile int*)&none = 1;
+    }
+    gather<DT>(list, static_cast<const T*>(P.z) + row * P.ld, P.list.top, 0, P.vocab);
+    list_softmax(list, P.list.top, P.c);
+  } else {
+    Stat st{-INFINITY, 0.f};
+    if (tid < sp.body - sp.lo) {
+      head = El<DT>::to(sp.row[sp.lo + tid]);
+      const float f[1] = {head};
+      absorb(st, f, P.c);
+    }
+    if (tid < sp.hi - sp.tail()) {
+      tail = El<DT>::to(sp.row[sp.tail() + tid]);
+      const float f[1] = {tail};
+      absorb(st, f, P.c);
+    }
+    for (int g = 0; g * U * kStream < sp.n_vec; ++g) {
+      copy_wait<D - 1>();
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = tid + (g * U + j) * kStream;
+        if (i < sp.n_vec) {
+          float f[V];
+          El<DT>::unpack(held[i], f);
+          absorb(st, f, P.c);
+        }
+      }
+      if (!*(volatile int*)&none) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          const int i = tid + ((g + D) * U + j) * kStream;
+          if (i < sp.n_vec) copy16(held + i, v + i);
+        }
+      }
+      copy_commit();
+    }
+    copy_wait<0>();
+    block_stat(st, P.c, red);
+  }
+  __syncthreads();
+  Stat st;
+  if (parts > 1) {
+    if (tid == 0) mine = total_of(red, kWarps, P.c);
+    __syncwarp();
+    st = cluster_stat(&mine, parts, P.c);
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this thread has read the peers' sums
+  } else {
+    st = total_of(red, kWarps, P.c);
+  }
+  const float B = P.g[row] * P.temperature, A = B + (P.g_lse ? P.g_lse[row] / P.temperature : 0.f);
+  T* out = static_cast<T*>(P.grad) + row * P.ld_grad;
+  const bool any = !none;
+  st = final_stat(st, bad);
+  if (tid >= kStream) {
+    if (part == 0) {
+      const float loss = list_loss(list, P.list.top, st, P.c, P.temperature);
+      if ((tid & 31) == 0) {
+        P.loss[row] = any ? (bad ? NAN : loss) : 0.f;
+        P.lse[row] = any ? st.m / P.temperature + logf(st.s) : 0.f;
+      }
+    }
+    list_sums(list, P.list.top);   // after the loss: it takes the place of log2 p
+  } else {
+    const float a = A / st.s;
+    const bool same = ((uintptr_t)(out + sp.body) & 15) == 0;
+    if (!any) {
+      for (int i = sp.lo + tid; i < sp.hi; i += kStream) out[i] = El<DT>::from(0.f);
+    } else {
+      uint4* o = reinterpret_cast<uint4*>(out + sp.body);
+      for (int i = tid; i < sp.n_vec; i += kStream) {
+        float f[V];
+        El<DT>::unpack(held[i], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[k] = dense<DT>(f[k], st.m, a, P.c);
+        if (same) {
+          __stcs(o + i, El<DT>::pack(f));
+        } else {
+          T* e = out + sp.body + i * V;
+#pragma unroll
+          for (int k = 0; k < V; ++k) e[k] = El<DT>::from(f[k]);
+        }
+      }
+      if (tid < sp.body - sp.lo) out[sp.lo + tid] = El<DT>::from(dense<DT>(head, st.m, a, P.c));
+      if (tid < sp.hi - sp.tail()) out[sp.tail() + tid] = El<DT>::from(dense<DT>(tail, st.m, a, P.c));
+    }
+  }
+  __syncthreads();
+  if (tid >= kStream && any) patch<DT>(list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // no CTA leaves while its sum may be read
 }
 
 int check_rows(const zt_distill_args* a, bool grad, const std::string& who) {
@@ -426,6 +560,35 @@ int backward(const zt_distill_args* a, cudaStream_t s, const char* who) {
   return launch(distill_backward_kernel<ZT_F32>, P, a->rows, false, 0, s, who);
 }
 
+// A part of distill_grad_kernel's row in shared memory: 64 KB leave room for three CTAs on an
+// SM, whose loads, sums and stores overlap; longer rows take up to kMaxPart in each of
+// eight parts, and rows beyond that the forward and the backward kernel.
+constexpr size_t kGoodPart = 64 * 1024;
+constexpr size_t kMaxPart = 200 * 1024;
+
+size_t part_bytes(const zt_distill_args* a, int parts) {
+  const size_t len = (size_t)(((a->vocab + parts - 1) / parts + 7) / 8 * 8);
+  return len * (a->dtype == ZT_F32 ? 4 : 2);
+}
+
+template <int DT> int grad_once(const RowsParams& P, int64_t rows, size_t smem, cudaStream_t s) {
+  static std::mutex mu;
+  static bool ready[64] = {false};
+  int dev = 0;
+  if (int rc = zt::check_cuda(cudaGetDevice(&dev), "zt_distill_rows_grad: cudaGetDevice")) return rc;
+  if (dev < 0 || dev >= 64) return zt::set_error(ZT_ERR_LIMIT, "zt_distill_rows_grad: device ordinal >= 64");
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!ready[dev]) {
+      if (int rc = zt::check_cuda(cudaFuncSetAttribute(distill_grad_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       (int)kMaxPart), "zt_distill_rows_grad: shared memory attribute"))
+        return rc;
+      ready[dev] = true;
+    }
+  }
+  return launch(distill_grad_kernel<DT>, P, rows, true, smem, s, "zt_distill_rows_grad launch");
+}
+
 }  // namespace
 
 extern "C" {
@@ -451,8 +614,18 @@ int zt_distill_rows_grad(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, true, "zt_distill_rows_grad")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->loss || !a->lse || !a->stats || !a->weight) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_grad: null pointer");
-  if (int rc = forward(a, zt::as_stream(stream), "zt_distill_rows_grad launch")) return rc;
-  return backward(a, zt::as_stream(stream), "zt_distill_rows_grad launch");
+  int parts = parts_for(a->rows, a->vocab);
+  while (parts < kMaxCluster && part_bytes(a, parts) > kGoodPart) parts *= 2;
+  const size_t smem = part_bytes(a, parts);
+  cudaStream_t s = zt::as_stream(stream);
+  if (smem > kMaxPart) {   // the row does not fit a cluster's shared memory
+    if (int rc = forward(a, s, "zt_distill_rows_grad launch")) return rc;
+    return backward(a, s, "zt_distill_rows_grad launch");
+  }
+  const RowsParams P = rows_params(a, parts);
+  if (a->dtype == ZT_BF16) return grad_once<ZT_BF16>(P, a->rows, smem, s);
+  if (a->dtype == ZT_F16) return grad_once<ZT_F16>(P, a->rows, smem, s);
+  return grad_once<ZT_F32>(P, a->rows, smem, s);
 }
 
 }  // extern "C"

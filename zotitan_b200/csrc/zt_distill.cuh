@@ -9,7 +9,6 @@ namespace zt {
 namespace distill {
 
 constexpr int kMaxTop = ZT_DISTILL_MAX_TOP;
-constexpr int kPer = kMaxTop / 32;   // list entries of a lane
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -85,82 +84,95 @@ struct TopList {
   const void* val;   // fp32, bf16 or fp16
   int32_t top, idx64, val_dtype;
   int64_t vocab;
-
-  __device__ __forceinline__ int64_t index(int64_t i) const {
-    return idx64 ? static_cast<const int64_t*>(idx)[i] : (int64_t)static_cast<const int32_t*>(idx)[i];
-  }
-  __device__ __forceinline__ float value(int64_t i) const {
-    if (val_dtype == ZT_F32) return static_cast<const float*>(val)[i];
-    if (val_dtype == ZT_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(val)[i]);
-    return __half2float(static_cast<const __half*>(val)[i]);
-  }
 };
 
-// One warp's view of a row's list: lane l holds entries l, l + 32, ... An entry with a
-// negative index or the value -inf carries no mass and its value is not looked at.
-struct Teacher {
-  int32_t idx[kPer];   // -1: no mass
-  float p[kPer];       // teacher probability
-  float lp[kPer];      // its log2 (0 where p is 0)
-  bool any;            // the row has a teacher
-  bool bad;            // an index >= vocab
+// A row's list in shared memory, worked on by one warp: lane l owns entries l, l + 32, ...
+// An entry with a negative index or the value -inf carries no mass and its other half is not
+// looked at.
+struct List {
+  int32_t idx[kMaxTop];   // -1: no mass
+  float p[kMaxTop];       // teacher probability, 0 without mass
+  float lp[kMaxTop];      // its log2, 0 where p is 0
+  float z[kMaxTop];       // the row's logit at idx
+};
 
-  __device__ __forceinline__ void read(const TopList& L, int64_t row) {
-    const int lane = threadIdx.x & 31;
-    bool some = false, out = false;
+struct Teacher {
+  bool any;   // the row has a teacher
+  bool bad;   // an index >= vocab
+};
+
+// The loads of four entries a lane are on their way before the first is looked at.
+template <class I, class F>
+__device__ __forceinline__ Teacher read_list(List& s, const I* __restrict__ idx, const F* __restrict__ val, int top, int64_t vocab) {
+  bool some = false, out = false;
+  for (int k0 = threadIdx.x & 31; k0 < top; k0 += 128) {
+    I i[4];
+    F v[4];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const int k = lane + 32 * e;
-      idx[e] = -1;
-      p[e] = -INFINITY;
-      if (32 * e < L.top && k < L.top) {
-        const int64_t i = L.index(row * L.top + k);
-        if (i >= 0) {
-          const float v = L.value(row * L.top + k);
-          if (!(v == -INFINITY)) {
-            some = true;
-            out = out || i >= L.vocab;
-            idx[e] = i < L.vocab ? (int32_t)i : -1;
-            p[e] = v;
-          }
-        }
+    for (int e = 0; e < 4; ++e) {
+      i[e] = -1;
+      if (k0 + 32 * e < top) {
+        i[e] = __ldg(idx + k0 + 32 * e);
+        v[e] = __ldg(val + k0 + 32 * e);
       }
     }
-    any = __any_sync(0xffffffffu, some);
-    bad = __any_sync(0xffffffffu, out);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k0 + 32 * e < top) {
+        const float f = (float)v[e];
+        const bool on = i[e] >= 0 && !(f == -INFINITY);
+        some = some || on;
+        out = out || (on && (int64_t)i[e] >= vocab);
+        s.idx[k0 + 32 * e] = on && (int64_t)i[e] < vocab ? (int32_t)i[e] : -1;
+        s.p[k0 + 32 * e] = on ? f : -INFINITY;
+      }
   }
+  Teacher t;
+  t.any = __any_sync(0xffffffffu, some);
+  t.bad = __any_sync(0xffffffffu, out);
+  return t;
+}
 
-  // p <- softmax of the values times c / log2(e) over the entries with mass
-  __device__ __forceinline__ void softmax(float c) {
-    float m = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) m = fmaxf(m, p[e]);
-    m = warp_max(m);
-    float t = 0.f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      lp[e] = (p[e] - m) * c;
-      p[e] = idx[e] >= 0 ? exp2f(lp[e]) : 0.f;
-      t += p[e];
-    }
-    t = warp_sum(t);
-    const float lt = log2f(t);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      p[e] = p[e] == 0.f ? 0.f : p[e] / t;   // a row without a teacher has t = 0
-      lp[e] = p[e] == 0.f ? 0.f : lp[e] - lt;
-    }
+template <class I> __device__ __forceinline__ Teacher read_list_as(List& s, const TopList& L, int64_t at) {
+  const I* i = static_cast<const I*>(L.idx) + at;
+  if (L.val_dtype == ZT_F32) return read_list(s, i, static_cast<const float*>(L.val) + at, L.top, L.vocab);
+  if (L.val_dtype == ZT_BF16) return read_list(s, i, static_cast<const __nv_bfloat16*>(L.val) + at, L.top, L.vocab);
+  return read_list(s, i, static_cast<const __half*>(L.val) + at, L.top, L.vocab);
+}
+
+__device__ __forceinline__ Teacher read_list(List& s, const TopList& L, int64_t row) {
+  if (L.idx64) return read_list_as<long long>(s, L, row * L.top);
+  return read_list_as<int32_t>(s, L, row * L.top);
+}
+
+// p <- softmax of the values times c / log2(e) over the entries with mass.
+__device__ __forceinline__ void list_softmax(List& s, int top, float c) {
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY;
+  for (int k = lane; k < top; k += 32) m = fmaxf(m, s.p[k]);
+  m = warp_max(m);
+  float t = 0.f;
+  for (int k = lane; k < top; k += 32) {
+    const float l = (s.p[k] - m) * c, p = s.idx[k] >= 0 ? exp2f(l) : 0.f;
+    s.lp[k] = l;
+    s.p[k] = p;
+    t += p;
   }
-};
+  t = warp_sum(t);
+  const float lt = log2f(t);
+  for (int k = lane; k < top; k += 32) {
+    const float p = s.p[k];   // a row without a teacher has t = 0
+    s.p[k] = p == 0.f ? 0.f : p / t;
+    s.lp[k] = p == 0.f ? 0.f : s.lp[k] - lt;
+  }
+}
 
 // T^2 sum_k p_k (log p_k - log q_k) from the list and the logits at its indices.
-__device__ __forceinline__ float list_loss(const Teacher& t, const float (&z)[kPer], const Stat& st, float c,
-                                           float temperature) {
+__device__ __forceinline__ float list_loss(const List& s, int top, const Stat& st, float c, float temperature) {
   const float ls = log2f(st.s);
   float a = 0.f;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e)
-    if (t.p[e] != 0.f) a = fmaf(t.p[e], t.lp[e] - ((z[e] - st.m) * c - ls), a);
+  for (int k = threadIdx.x & 31; k < top; k += 32)
+    if (s.p[k] != 0.f) a = fmaf(s.p[k], s.lp[k] - ((s.z[k] - st.m) * c - ls), a);
   return warp_sum(a) * (kLn2 * temperature * temperature);
 }
 

@@ -16,7 +16,7 @@
 //    A listed logit is fetched by a one-column load of tensor memory at that column (the
 //    column is the same for the warp's 32 rows, so a warp makes one such load per listed
 //    (row, token) of its rows and tile: about four at 64 entries of 128256 tokens).
-// 3. combine_kernel, a warp per row: the splits' sums in vocabulary order, then the list.
+// 3. combine_kernel: a row's sums over the splits, then its list.
 // Every mbarrier wait is bounded; on expiry the kernel records an error
 // (zt_linear_distill_take_error), drains its own copies and MMAs and frees its tensor memory.
 #include <math.h>
@@ -65,33 +65,23 @@ __global__ void __launch_bounds__(32 * kListWarps) list_kernel(const __grid_cons
   const int64_t row = (int64_t)blockIdx.x * kListWarps + threadIdx.x / 32;
   if (row >= P.rows) return;
   const int lane = threadIdx.x & 31;
-  Teacher t;
-  t.read(P.list, row);
-  t.softmax(P.c);
-  int32_t key[kPer], rank[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    key[e] = t.p[e] != 0.f ? t.idx[e] : INT32_MAX;
-    rank[e] = 0;
+  __shared__ List lists[kListWarps];
+  List& s = lists[threadIdx.x / 32];
+  const Teacher t = read_list(s, P.list, row);
+  list_softmax(s, P.top, P.c);
+  for (int k = lane; k < P.top; k += 32)
+    if (s.p[k] == 0.f) s.idx[k] = INT32_MAX;   // no mass: behind the others
+  __syncwarp();
+  // an entry's place: those with a smaller token, or the same and an earlier place
+  for (int k = lane; k < P.top; k += 32) {
+    const int32_t own = s.idx[k];
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < P.top; ++j) place += (s.idx[j] < own || (s.idx[j] == own && j < k)) ? 1 : 0;
+    const int64_t at = row * P.top + place;
+    P.idx[at] = own;
+    P.lp[at] = s.lp[k];
   }
-  // rank of entry (e, lane): entries with a smaller token, or the same and an earlier place
-#pragma unroll
-  for (int o = 0; o < kPer; ++o) {
-    if (32 * o >= P.top) break;
-    for (int l = 0; l < 32; ++l) {
-      const int32_t other = __shfl_sync(0xffffffffu, key[o], l);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (32 * e < P.top) rank[e] += (other < key[e] || (other == key[e] && (o < e || (o == e && l < lane)))) ? 1 : 0;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < kPer; ++e)
-    if (lane + 32 * e < P.top) {
-      const int64_t at = row * P.top + rank[e];
-      P.idx[at] = key[e];
-      P.lp[at] = t.lp[e];
-    }
   if (lane == 0) P.status[row] = !t.any ? kNoTeacher : t.bad ? kBadIndex : kHasTeacher;
 }
 
@@ -297,28 +287,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
+// 32 rows a block. Warp w merges splits w, w + kListWarps, ... of the rows, lane = row, so that
+// a warp reads 256 adjacent bytes; then each warp takes the lists of four rows.
 __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_constant__ Params P) {
-  const int64_t row = (int64_t)blockIdx.x * kListWarps + threadIdx.x / 32;
-  if (row >= P.rows) return;
-  const int lane = threadIdx.x & 31;
+  __shared__ Stat part[kListWarps][32];
+  const int64_t row0 = (int64_t)blockIdx.x * 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   Stat st{-INFINITY, 0.f};
-  for (int sp = lane; sp < P.n_splits; sp += 32) {
-    const float2 o = P.partials[(size_t)sp * P.rows_pad + row];
+#pragma unroll 4
+  for (int sp = warp; sp < P.n_splits; sp += kListWarps) {   // rows_pad covers row0 + lane
+    const float2 o = P.partials[(size_t)sp * P.rows_pad + row0 + lane];
     st = merge(st, Stat{o.x, o.y}, P.c);
   }
-  st = warp_merge(st, P.c);
-  if (st.m == -INFINITY) st.s = NAN;
-  const float ls = log2f(st.s);
-  float a = 0.f;
-  for (int k = lane; k < P.top; k += 32) {
-    const int64_t at = row * P.top + k;
-    if (P.idx[at] != INT32_MAX) a = fmaf(exp2f(P.lp[at]), P.lp[at] - ((P.z[at] - st.m) * P.c - ls), a);
-  }
-  a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
-  if (lane == 0) {
-    const int32_t status = P.status[row];
-    P.loss[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : a;
-    P.lse[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : st.m / P.temperature + logf(st.s);
+  part[warp][lane] = st;
+  __syncthreads();
+  for (int r = warp; r < 32; r += kListWarps) {
+    const int64_t row = row0 + r;
+    if (row >= P.rows) break;
+    st = part[0][r];
+#pragma unroll
+    for (int w = 1; w < kListWarps; ++w) st = merge(st, part[w][r], P.c);
+    if (st.m == -INFINITY) st.s = NAN;
+    const float ls = log2f(st.s);
+    float a = 0.f;
+    for (int k = lane; k < P.top; k += 32) {
+      const int64_t at = row * P.top + k;
+      if (P.idx[at] != INT32_MAX) a = fmaf(exp2f(P.lp[at]), P.lp[at] - ((P.z[at] - st.m) * P.c - ls), a);
+    }
+    a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
+    if (lane == 0) {
+      const int32_t status = P.status[row];
+      P.loss[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : a;
+      P.lse[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : st.m / P.temperature + logf(st.s);
+    }
   }
 }
 
@@ -475,7 +476,7 @@ int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
   if (int rc = zt::check_cuda(cudaGetLastError(), "zt_linear_distill: list launch")) return rc;
   linear_distill_kernel<<<2 * clusters, kThreads, kSmem, s>>>(P);
   if (int rc = zt::check_cuda(cudaGetLastError(), "zt_linear_distill: gemm launch")) return rc;
-  combine_kernel<<<row_blocks, 32 * kListWarps, 0, s>>>(P);
+  combine_kernel<<<(unsigned)((a->rows + 31) / 32), 32 * kListWarps, 0, s>>>(P);
   return zt::check_cuda(cudaGetLastError(), "zt_linear_distill: combine launch");
 }
 

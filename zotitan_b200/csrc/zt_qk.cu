@@ -19,12 +19,18 @@
 // once and keeps packed in registers.
 #include <math.h>
 
+#include <mutex>
+
 #include "zt_common.cuh"
 
 namespace {
 
 constexpr int kWarps = 4;          // warps of a forward block; they share nothing
 constexpr int kBwdWarps = 8;       // warps of a backward block; they share the weight gradient's sum
+constexpr int kBwdBlocks = 2;      // of them on an SM
+constexpr int kFwdBlocks = 5;      // ring kernels: forward blocks on an SM, and the steps a warp has in flight
+constexpr int kFwdRing = 8;
+constexpr int kBwdRing = 4;
 constexpr int kMaxHeadDim = 512;   // 32 lanes x 8 elements of each half
 constexpr int kE = 8;              // elements of each half that a lane holds at most
 
@@ -91,6 +97,9 @@ template <int DT, int V, int NC> struct Piece {
       }
     }
   }
+  __device__ __forceinline__ void take(const uint4& u) {
+    w[0][0] = u.x; w[0][1] = u.y; w[0][2] = u.z; w[0][3] = u.w;
+  }
   __device__ __forceinline__ float at(int c, int j) const {
     if constexpr (DT == ZT_F32) {
       return __uint_as_float(w[c][j]);
@@ -110,216 +119,153 @@ __device__ __forceinline__ void store_piece(typename El<DT>::T* p, const float (
   for (int c = 0; c < NC; ++c) {
     const int i = (c * lanes + sub) * V;
     if (i >= half) continue;
-    if constexpr (V * sizeof(T) == 16) {
-      uint4 u;
-      if constexpr (DT == ZT_F32) {
-        u = make_uint4(__float_as_uint(v[c][0]), __float_as_uint(v[c][1]), __float_as_uint(v[c][2]), __float_as_uint(v[c][3]));
-      } else if constexpr (DT == ZT_BF16) {
-        uint32_t r[4];
+    if constexpr (V == 4 && DT == ZT_F32) {
+      *reinterpret_cast<float4*>(p + i) = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
+    } else if constexpr (V == 8) {
+      uint32_t r[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (DT == ZT_BF16) {
           const __nv_bfloat162 h = __floats2bfloat162_rn(v[c][2 * j], v[c][2 * j + 1]);
           r[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        u = make_uint4(r[0], r[1], r[2], r[3]);
-      } else {
-        uint32_t r[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        } else {
           const __half2 h = __floats2half2_rn(v[c][2 * j], v[c][2 * j + 1]);
           r[j] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        u = make_uint4(r[0], r[1], r[2], r[3]);
       }
-      *reinterpret_cast<uint4*>(p + i) = u;
+      *reinterpret_cast<uint4*>(p + i) = make_uint4(r[0], r[1], r[2], r[3]);
     } else {
       p[i] = El<DT>::from(v[c][0]);
     }
   }
 }
 
-// Weights and tables: packed in the heads' own type (SAME), or of either type, widened to
-// fp32 as they are loaded.
-template <int DT, int V, int NC, bool SAME> struct Side;
-template <int DT, int V, int NC> struct Side<DT, V, NC, true> {
-  Piece<DT, V, NC> lo, hi;
-  __device__ __forceinline__ void load(const void* base, int64_t off, int32_t, int sub, int lanes, int half) {
-    const typename El<DT>::T* p = static_cast<const typename El<DT>::T*>(base) + off;
-    lo.load(p, sub, lanes, half);
-    hi.load(p + half, sub, lanes, half);
-  }
-  __device__ __forceinline__ float l(int c, int j) const { return lo.at(c, j); }
-  __device__ __forceinline__ float h(int c, int j) const { return hi.at(c, j); }
-};
-template <int DT, int V, int NC> struct Side<DT, V, NC, false> {
-  float lo[NC][V], hi[NC][V];
-  __device__ __forceinline__ static float one(const void* base, int64_t i, int32_t dtype) {
-    if (dtype == ZT_F32) return static_cast<const float*>(base)[i];
-    return El<DT>::to(static_cast<const typename El<DT>::T*>(base)[i]);
-  }
-  __device__ __forceinline__ void load(const void* base, int64_t off, int32_t dtype, int sub, int lanes, int half) {
+// A lane's V elements of a weight or table row, of the heads' type or fp32, as fp32.
+template <int DT, int V, int NC>
+__device__ __forceinline__ void load_side(float (&v)[NC][V], const void* base, int64_t off, int32_t dtype, int sub, int lanes,
+                                          int half) {
+  using T = typename El<DT>::T;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int i = (c * lanes + sub) * V;
+  for (int c = 0; c < NC; ++c) {
+    const int i = (c * lanes + sub) * V;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        lo[c][j] = i + j < half ? one(base, off + i + j, dtype) : 0.f;
-        hi[c][j] = i + j < half ? one(base, off + half + i + j, dtype) : 0.f;
+    for (int j = 0; j < V; ++j) v[c][j] = 0.f;
+    if (i >= half) continue;
+    if (DT != ZT_F32 && dtype == ZT_F32) {
+      const float* p = static_cast<const float*>(base) + off + i;
+      if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int q = 0; q < V; q += 4) {
+          const float4 u = *reinterpret_cast<const float4*>(p + q);
+          v[c][q] = u.x; v[c][q + 1] = u.y; v[c][q + 2] = u.z; v[c][q + 3] = u.w;
+        }
+      } else {
+        v[c][0] = *p;
       }
+    } else {
+      Piece<DT, V, 1> u;
+      u.load(static_cast<const T*>(base) + off + i, 0, 1, V);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[c][j] = u.at(0, j);
     }
   }
-  __device__ __forceinline__ float l(int c, int j) const { return lo[c][j]; }
-  __device__ __forceinline__ float h(int c, int j) const { return hi[c][j]; }
-};
+}
 
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+// Sum over the lanes of a head; LANES = 0: known at run time only.
+template <int LANES> __device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  if constexpr (LANES > 0) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  } else {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
   return v;
 }
 
-// One warp: position `row`, its head groups part, part + split, ...
-template <int DT, int V, int NC, bool SAME>
+// A warp's part of the groups [0, groups) of q or k, whose first lies `before` groups into
+// the position's: those congruent to `part` modulo `split`.
+__device__ __forceinline__ int first_of(int before, int part, int split) {
+  return part >= before ? part - before : (split - (before - part) % split) % split;
+}
+
+// ---- the plain kernels: single elements -------------------------------------------------------
+//
+// One warp a position and part of its heads. Weight, cos and sin enter as their products
+// (w cos and w' sin, once per position), and n at the end:
+//   out[i] = n (x[i] (w[i] cos[i]) - x[i + h] (w[i + h] sin[i])), out[i + h] alike.
+template <int DT>
 __global__ void __launch_bounds__(32 * kWarps) qk_forward_kernel(const __grid_constant__ QkParams P) {
   using T = typename El<DT>::T;
+  constexpr int V = 1, NC = kE;
   const int64_t item = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
   if (item >= (int64_t)P.rows * P.split) return;
   const int row = (int)(item / P.split), part = (int)(item - (int64_t)row * P.split);
-  const int lane = threadIdx.x & 31;
-  const int sub = lane & (P.lanes - 1), mine = lane / P.lanes, per_warp = 32 / P.lanes;
+  const int lanes = P.lanes, per_warp = 32 / lanes;
+  const int lane = threadIdx.x & 31, sub = lane & (lanes - 1), mine = lane / lanes;
   const int b = row / P.seq, t = row - b * P.seq;
   const int64_t trow = (int64_t)(P.per_batch ? row : t) * P.hd;
-
-  Side<DT, V, NC, SAME> cs, sn, w;
-  cs.load(P.cos, trow, P.t_dtype, sub, P.lanes, P.half);
-  sn.load(P.sin, trow, P.t_dtype, sub, P.lanes, P.half);
-  const int total = P.groups[0] + P.groups[1];
-  int loaded = -1;
-  for (int grp = part; grp < total; grp += P.split) {
-    const int which = grp >= P.groups[0];
-    const int head = (grp - (which ? P.groups[0] : 0)) * per_warp + mine;
-    const bool on = head < P.heads[which];
-    if (which != loaded) {
-      w.load(P.w[which], 0, P.w_dtype, sub, P.lanes, P.half);
-      loaded = which;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    int grp = first_of(which ? P.groups[0] : 0, part, P.split);
+    if (grp >= P.groups[which]) continue;
+    float ac[NC][V], as[NC][V], bc[NC][V], bs[NC][V];   // w cos, w' sin of the first half; w' cos', w sin' of the second
+    {
+      float wl[NC][V], wh[NC][V];
+      load_side<DT, V, NC>(wl, P.w[which], 0, P.w_dtype, sub, lanes, P.half);
+      load_side<DT, V, NC>(wh, P.w[which], P.half, P.w_dtype, sub, lanes, P.half);
+      load_side<DT, V, NC>(ac, P.cos, trow, P.t_dtype, sub, lanes, P.half);
+      load_side<DT, V, NC>(bc, P.cos, trow + P.half, P.t_dtype, sub, lanes, P.half);
+      load_side<DT, V, NC>(as, P.sin, trow, P.t_dtype, sub, lanes, P.half);
+      load_side<DT, V, NC>(bs, P.sin, trow + P.half, P.t_dtype, sub, lanes, P.half);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        ac[c][0] *= wl[c][0];
+        as[c][0] *= wh[c][0];
+        bc[c][0] *= wh[c][0];
+        bs[c][0] *= wl[c][0];
+      }
     }
-    Piece<DT, V, NC> lo, hi;
-    const T* x = static_cast<const T*>(P.x[which]) + b * P.xs[which][0] + t * P.xs[which][1] + head * P.xs[which][2];
-    lo.load(x, sub, P.lanes, on ? P.half : 0);
-    hi.load(x + P.half, sub, P.lanes, on ? P.half : 0);
-    float ss = 0.f;
+    for (; grp < P.groups[which]; grp += P.split) {
+      const int head = grp * per_warp + mine;
+      const bool on = head < P.heads[which];
+      const T* x = static_cast<const T*>(P.x[which]) + b * P.xs[which][0] + t * P.xs[which][1] + head * P.xs[which][2];
+      Piece<DT, V, NC> lo, hi;
+      lo.load(x, sub, lanes, on ? P.half : 0);
+      hi.load(x + P.half, sub, lanes, on ? P.half : 0);
+      float ss = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        ss = fmaf(lo.at(c, j), lo.at(c, j), ss);
-        ss = fmaf(hi.at(c, j), hi.at(c, j), ss);
+      for (int c = 0; c < NC; ++c) {
+        ss = fmaf(lo.at(c, 0), lo.at(c, 0), ss);
+        ss = fmaf(hi.at(c, 0), hi.at(c, 0), ss);
       }
-    const float n = rsqrtf(fmaf(lanes_sum(ss, P.lanes), P.inv_hd, P.eps));
-    float ol[NC][V], oh[NC][V];
+      const float n = rsqrtf(fmaf(lanes_sum<0>(ss, lanes), P.inv_hd, P.eps));
+      float ol[NC][V], oh[NC][V];
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float yl = lo.at(c, j) * n * w.l(c, j), yh = hi.at(c, j) * n * w.h(c, j);
-        ol[c][j] = fmaf(yl, cs.l(c, j), -yh * sn.l(c, j));
-        oh[c][j] = fmaf(yh, cs.h(c, j), yl * sn.h(c, j));
+      for (int c = 0; c < NC; ++c) {
+        const float xl = lo.at(c, 0), xh = hi.at(c, 0);
+        ol[c][0] = n * fmaf(xl, ac[c][0], -xh * as[c][0]);
+        oh[c][0] = n * fmaf(xh, bc[c][0], xl * bs[c][0]);
       }
-    if (on) {
-      T* o = static_cast<T*>(P.out[which]) + b * P.os[which][0] + t * P.os[which][1] + head * P.os[which][2];
-      store_piece<DT, V, NC>(o, ol, sub, P.lanes, P.half);
-      store_piece<DT, V, NC>(o + P.half, oh, sub, P.lanes, P.half);
+      if (on) {
+        T* o = static_cast<T*>(P.out[which]) + b * P.os[which][0] + t * P.os[which][1] + head * P.os[which][2];
+        store_piece<DT, V, NC>(o, ol, sub, lanes, P.half);
+        store_piece<DT, V, NC>(o + P.half, oh, sub, lanes, P.half);
+      }
     }
   }
 }
 
-// Persistent warps over (position, part of its heads); each lane sums its elements of the
-// weight gradients in registers, a block adds its warps' sums in warp order.
-template <int DT, int V, int NC, bool SAME>
-__global__ void __launch_bounds__(32 * kBwdWarps) qk_backward_kernel(const __grid_constant__ QkParams P) {
-  using T = typename El<DT>::T;
-  extern __shared__ float sums[];   // [kBwdWarps][2][hd]
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int sub = lane & (P.lanes - 1), mine = lane / P.lanes, per_warp = 32 / P.lanes;
-  const int total = P.groups[0] + P.groups[1];
-  float dl[2][NC][V], dh[2][NC][V];
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < V; ++j) dl[a][c][j] = dh[a][c][j] = 0.f;
-
-  const int64_t items = (int64_t)P.rows * P.split;
-  for (int64_t item = (int64_t)blockIdx.x * kBwdWarps + warp; item < items; item += (int64_t)gridDim.x * kBwdWarps) {
-    const int row = (int)(item / P.split), part = (int)(item - (int64_t)row * P.split);
-    const int b = row / P.seq, t = row - b * P.seq;
-    const int64_t trow = (int64_t)(P.per_batch ? row : t) * P.hd;
-    Side<DT, V, NC, SAME> cs, sn, w;
-    cs.load(P.cos, trow, P.t_dtype, sub, P.lanes, P.half);
-    sn.load(P.sin, trow, P.t_dtype, sub, P.lanes, P.half);
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int first = which ? P.groups[0] : 0, last = which ? total : P.groups[0];
-      // the first group of this part at or after `first`
-      int grp = part >= first ? part : part + (first - part + P.split - 1) / P.split * P.split;
-      if (grp >= last) continue;
-      w.load(P.w[which], 0, P.w_dtype, sub, P.lanes, P.half);
-      for (; grp < last; grp += P.split) {
-        const int head = (grp - first) * per_warp + mine;
-        const bool on = head < P.heads[which];
-        const T* x = static_cast<const T*>(P.x[which]) + b * P.xs[which][0] + t * P.xs[which][1] + head * P.xs[which][2];
-        const T* g = static_cast<const T*>(P.g[which]) + b * P.gs[which][0] + t * P.gs[which][1] + head * P.gs[which][2];
-        Piece<DT, V, NC> xl, xh, gl, gh;
-        xl.load(x, sub, P.lanes, on ? P.half : 0);
-        xh.load(x + P.half, sub, P.lanes, on ? P.half : 0);
-        gl.load(g, sub, P.lanes, on ? P.half : 0);
-        gh.load(g + P.half, sub, P.lanes, on ? P.half : 0);
-        float ss = 0.f, sd = 0.f;
-        float yl[NC][V], yh[NC][V];
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float a = xl.at(c, j), z = xh.at(c, j);
-            ss = fmaf(a, a, ss);
-            ss = fmaf(z, z, ss);
-            yl[c][j] = fmaf(gl.at(c, j), cs.l(c, j), gh.at(c, j) * sn.h(c, j));
-            yh[c][j] = fmaf(gh.at(c, j), cs.h(c, j), -gl.at(c, j) * sn.l(c, j));
-            sd = fmaf(yl[c][j] * w.l(c, j), a, sd);
-            sd = fmaf(yh[c][j] * w.h(c, j), z, sd);
-          }
-        ss = lanes_sum(ss, P.lanes);
-        sd = lanes_sum(sd, P.lanes);
-        const float n = rsqrtf(fmaf(ss, P.inv_hd, P.eps));
-        const float m = n * n * sd * P.inv_hd;   // dx = n (w dy - x m)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float a = xl.at(c, j), z = xh.at(c, j);
-            if (on) {   // a head that is not there has no x to be finite
-              dl[which][c][j] = fmaf(yl[c][j], a * n, dl[which][c][j]);
-              dh[which][c][j] = fmaf(yh[c][j], z * n, dh[which][c][j]);
-            }
-            yl[c][j] = n * fmaf(-a, m, yl[c][j] * w.l(c, j));
-            yh[c][j] = n * fmaf(-z, m, yh[c][j] * w.h(c, j));
-          }
-        if (on) {
-          T* o = static_cast<T*>(P.out[which]) + b * P.os[which][0] + t * P.os[which][1] + head * P.os[which][2];
-          store_piece<DT, V, NC>(o, yl, sub, P.lanes, P.half);
-          store_piece<DT, V, NC>(o + P.half, yh, sub, P.lanes, P.half);
-        }
-      }
-    }
-  }
-  // lanes of the same elements in a warp, then the block's warps
+// A block's weight gradients: lanes of the same elements in a warp, then the warps in order.
+template <int V, int NC>
+__device__ __forceinline__ void block_weights(const QkParams& P, float (&dl)[2][NC][V], float (&dh)[2][NC][V], float* sums, int warp,
+                                              int lanes, int sub, int mine) {
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        for (int o = P.lanes; o < 32; o <<= 1) {
+        for (int o = lanes; o < 32; o <<= 1) {
           dl[a][c][j] += __shfl_xor_sync(0xffffffffu, dl[a][c][j], o);
           dh[a][c][j] += __shfl_xor_sync(0xffffffffu, dh[a][c][j], o);
         }
@@ -330,7 +276,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps) qk_backward_kernel(const __gri
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const int i = (c * P.lanes + sub) * V + j;
+          const int i = (c * lanes + sub) * V + j;
           if (i < P.half) {
             sums[(warp * 2 + a) * P.hd + i] = dl[a][c][j];
             sums[(warp * 2 + a) * P.hd + P.half + i] = dh[a][c][j];
@@ -346,50 +292,445 @@ __global__ void __launch_bounds__(32 * kBwdWarps) qk_backward_kernel(const __gri
   }
 }
 
-// The blocks' weight gradients, summed in block order by 8 x 32 threads per 32 columns and
+// Persistent warps over (position, part of its heads); each lane sums its elements of the
+// weight gradients in registers, a block adds its warps' sums in warp order.
+template <int DT>
+__global__ void __launch_bounds__(32 * kBwdWarps) qk_backward_kernel(const __grid_constant__ QkParams P) {
+  using T = typename El<DT>::T;
+  constexpr int V = 1, NC = kE;
+  extern __shared__ float sums[];   // [kBwdWarps][2][hd]
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int lanes = P.lanes, per_warp = 32 / lanes, sub = lane & (lanes - 1), mine = lane / lanes;
+  float dl[2][NC][V], dh[2][NC][V];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) dl[a][c][0] = dh[a][c][0] = 0.f;
+
+  const int64_t items = (int64_t)P.rows * P.split;
+  for (int64_t item = (int64_t)blockIdx.x * kBwdWarps + warp; item < items; item += (int64_t)gridDim.x * kBwdWarps) {
+    const int row = (int)(item / P.split), part = (int)(item - (int64_t)row * P.split);
+    const int b = row / P.seq, t = row - b * P.seq;
+    const int64_t trow = (int64_t)(P.per_batch ? row : t) * P.hd;
+    float cl[NC][V], ch[NC][V], sl[NC][V], sh[NC][V];
+    load_side<DT, V, NC>(cl, P.cos, trow, P.t_dtype, sub, lanes, P.half);
+    load_side<DT, V, NC>(ch, P.cos, trow + P.half, P.t_dtype, sub, lanes, P.half);
+    load_side<DT, V, NC>(sl, P.sin, trow, P.t_dtype, sub, lanes, P.half);
+    load_side<DT, V, NC>(sh, P.sin, trow + P.half, P.t_dtype, sub, lanes, P.half);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      int grp = first_of(which ? P.groups[0] : 0, part, P.split);
+      if (grp >= P.groups[which]) continue;
+      float wl[NC][V], wh[NC][V];
+      load_side<DT, V, NC>(wl, P.w[which], 0, P.w_dtype, sub, lanes, P.half);
+      load_side<DT, V, NC>(wh, P.w[which], P.half, P.w_dtype, sub, lanes, P.half);
+      for (; grp < P.groups[which]; grp += P.split) {
+        const int head = grp * per_warp + mine;
+        const bool on = head < P.heads[which];
+        const T* x = static_cast<const T*>(P.x[which]) + b * P.xs[which][0] + t * P.xs[which][1] + head * P.xs[which][2];
+        const T* g = static_cast<const T*>(P.g[which]) + b * P.gs[which][0] + t * P.gs[which][1] + head * P.gs[which][2];
+        Piece<DT, V, NC> xl, xh, gl, gh;
+        xl.load(x, sub, lanes, on ? P.half : 0);
+        xh.load(x + P.half, sub, lanes, on ? P.half : 0);
+        gl.load(g, sub, lanes, on ? P.half : 0);
+        gh.load(g + P.half, sub, lanes, on ? P.half : 0);
+        float ss = 0.f, sd = 0.f;
+        float yl[NC][V], yh[NC][V];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float a = xl.at(c, 0), z = xh.at(c, 0);
+          ss = fmaf(a, a, ss);
+          ss = fmaf(z, z, ss);
+          yl[c][0] = fmaf(gl.at(c, 0), cl[c][0], gh.at(c, 0) * sh[c][0]);
+          yh[c][0] = fmaf(gh.at(c, 0), ch[c][0], -gl.at(c, 0) * sl[c][0]);
+          sd = fmaf(yl[c][0] * wl[c][0], a, sd);
+          sd = fmaf(yh[c][0] * wh[c][0], z, sd);
+        }
+        ss = lanes_sum<0>(ss, lanes);
+        sd = lanes_sum<0>(sd, lanes);
+        if (on) {   // a head that is not there has no x to be finite
+          const float n = rsqrtf(fmaf(ss, P.inv_hd, P.eps));
+          const float m = n * n * sd * P.inv_hd;   // dx = n w dy - (x n) m
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const float a = xl.at(c, 0) * n, z = xh.at(c, 0) * n;
+            dl[which][c][0] = fmaf(yl[c][0], a, dl[which][c][0]);
+            dh[which][c][0] = fmaf(yh[c][0], z, dh[which][c][0]);
+            yl[c][0] = fmaf(-a, m, n * (yl[c][0] * wl[c][0]));
+            yh[c][0] = fmaf(-z, m, n * (yh[c][0] * wh[c][0]));
+          }
+          T* o = static_cast<T*>(P.out[which]) + b * P.os[which][0] + t * P.os[which][1] + head * P.os[which][2];
+          store_piece<DT, V, NC>(o, yl, sub, lanes, P.half);
+          store_piece<DT, V, NC>(o + P.half, yh, sub, lanes, P.half);
+        }
+      }
+    }
+  }
+  block_weights<V, NC>(P, dl, dh, sums, warp, lanes, sub, mine);
+}
+
+// ---- the ring kernels: 16 bytes of a head a lane ---------------------------------------------
+//
+// The kernels above wait for memory several times a position (tables, then each step's heads), and
+// the registers that their loads land in bound the warps of an SM. Here a warp walks many
+// positions and copies the heads of the next steps to its own ring in shared memory (cp.async;
+// a lane reads back only what it copied itself, so no barrier is needed).
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 smem_load16(uint32_t src) {
+  uint4 u;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(src) : "memory");
+  return u;
+}
+__device__ __forceinline__ void smem_store16(uint32_t dst, const float* v) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+}
+// A lane's V fp32 values, 512 bytes (a warp's 16) apart every four.
+template <int V> __device__ __forceinline__ void smem_get(float (&v)[V], uint32_t src) {
+#pragma unroll
+  for (int q = 0; q < V; q += 4) {
+    const uint4 u = smem_load16(src + q * 128);
+    v[q] = __uint_as_float(u.x); v[q + 1] = __uint_as_float(u.y); v[q + 2] = __uint_as_float(u.z); v[q + 3] = __uint_as_float(u.w);
+  }
+}
+template <int V> __device__ __forceinline__ void smem_put(uint32_t dst, const float (&v)[V]) {
+#pragma unroll
+  for (int q = 0; q < V; q += 4) smem_store16(dst + q * 128, v + q);
+}
+
+// Item i of a launch: a position and a part of its heads (rows x split stays below 2^26).
+struct Item {
+  int row, part, b, t;
+  __device__ __forceinline__ Item(const QkParams& P, int i) {
+    row = P.split == 1 ? i : (int)((uint32_t)i / (uint32_t)P.split);
+    part = P.split == 1 ? 0 : i - row * P.split;
+    b = (int)((uint32_t)row / (uint32_t)P.seq);
+    t = row - b * P.seq;
+  }
+  template <class T> __device__ __forceinline__ T* at(T* base, const int64_t (&s)[3], int head) const {
+    return base + b * s[0] + t * s[1] + head * s[2];
+  }
+};
+
+// Walks a warp's steps: items from `item` on in strides of `stride`, in each the part's groups of
+// q, then of k. The pointers are the lane's own.
+template <class T, bool GRAD> struct Cursor {
+  int item, items, stride;
+  int which, head, left;   // the lane's head, and the groups left in this section
+  const T *x, *g;
+
+  // The part's first group of q (w = 0) or k of the current item, or of a later one.
+  __device__ __forceinline__ void enter(const QkParams& P, int w, int per_warp, int mine, int at) {
+    while (item < items) {
+      const Item it(P, item);
+#pragma unroll 1
+      for (; w < 2; ++w) {
+        const int grp = first_of(w ? P.groups[0] : 0, it.part, P.split);
+        if (grp < P.groups[w]) {
+          which = w;
+          left = P.split == 1 ? P.groups[w] : (P.groups[w] - grp + P.split - 1) / P.split;
+          head = grp * per_warp + mine;
+          x = it.at(static_cast<const T*>(P.x[w]), P.xs[w], head) + at;
+          if (GRAD) g = it.at(static_cast<const T*>(P.g[w]), P.gs[w], head) + at;
+          return;
+        }
+      }
+      item += stride;
+      w = 0;
+    }
+  }
+  __device__ __forceinline__ void advance(const QkParams& P, int per_warp, int mine, int at) {
+    if (--left > 0) {
+      const int hstep = per_warp * P.split;
+      head += hstep;
+      x += hstep * P.xs[which][2];
+      if (GRAD) g += hstep * P.gs[which][2];
+    } else {
+      const int w = which + 1;
+      if (w == 2) item += stride;
+      enter(P, w & 1, per_warp, mine, at);
+    }
+  }
+};
+
+template <int DT, int LANES>
+__global__ void __launch_bounds__(32 * kWarps, kFwdBlocks) qk_forward_ring_kernel(const __grid_constant__ QkParams P) {
+  using T = typename El<DT>::T;
+  constexpr int V = 16 / (int)sizeof(T), D = kFwdRing;
+  __shared__ uint4 rings[kWarps][D][2][32];
+  const int lanes = LANES > 0 ? LANES : P.lanes, per_warp = 32 / lanes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, sub = lane & (lanes - 1), mine = lane / lanes;
+  const uint32_t ring = smem_at(&rings[warp][0][0][lane]);   // a step's slot is 1024 bytes
+  const bool in = sub * V < P.half;
+  Cursor<T, false> ahead;
+  ahead.item = blockIdx.x * kWarps + warp;
+  ahead.items = P.rows * P.split;
+  ahead.stride = gridDim.x * kWarps;
+  ahead.enter(P, 0, per_warp, mine, sub * V);
+  auto fetch = [&](uint32_t slot) {
+    if (ahead.item < ahead.items) {
+      if (in && ahead.head < P.heads[ahead.which]) {
+        copy16(slot, ahead.x);
+        copy16(slot + 512, ahead.x + P.half);
+      }
+      ahead.advance(P, per_warp, mine, sub * V);
+    }
+    copy_commit();
+  };
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) fetch(ring + d * 1024);
+  int slot = 0;
+  const int items = ahead.items, stride = ahead.stride;
+  for (int item = blockIdx.x * kWarps + warp; item < items; item += stride) {
+    const Item it(P, item);
+    const int64_t trow = (int64_t)(P.per_batch ? it.row : it.t) * P.hd;
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      int grp = first_of(which ? P.groups[0] : 0, it.part, P.split);
+      if (grp >= P.groups[which]) continue;
+      float ac[1][V], as[1][V], bc[1][V], bs[1][V];   // w cos, w' sin of the first half; w' cos', w sin' of the second
+      {
+        float wl[1][V], wh[1][V];
+        load_side<DT, V, 1>(wl, P.w[which], 0, P.w_dtype, sub, lanes, P.half);
+        load_side<DT, V, 1>(wh, P.w[which], P.half, P.w_dtype, sub, lanes, P.half);
+        load_side<DT, V, 1>(ac, P.cos, trow, P.t_dtype, sub, lanes, P.half);
+        load_side<DT, V, 1>(bc, P.cos, trow + P.half, P.t_dtype, sub, lanes, P.half);
+        load_side<DT, V, 1>(as, P.sin, trow, P.t_dtype, sub, lanes, P.half);
+        load_side<DT, V, 1>(bs, P.sin, trow + P.half, P.t_dtype, sub, lanes, P.half);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          ac[0][j] *= wl[0][j];
+          as[0][j] *= wh[0][j];
+          bc[0][j] *= wh[0][j];
+          bs[0][j] *= wl[0][j];
+        }
+      }
+      const int hstep = per_warp * P.split, heads = P.heads[which];
+      int head = grp * per_warp + mine;
+      T* o = it.at(static_cast<T*>(P.out[which]), P.os[which], head) + sub * V;
+      const int64_t ostep = hstep * P.os[which][2];
+      for (; grp < P.groups[which]; grp += P.split) {
+        const bool on = in && head < heads;
+        const uint32_t here = ring + slot * 1024;
+        copy_wait<D - 1>();
+        Piece<DT, V, 1> lo, hi;
+        lo.take(smem_load16(here));
+        hi.take(smem_load16(here + 512));
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          ss = fmaf(lo.at(0, j), lo.at(0, j), ss);
+          ss = fmaf(hi.at(0, j), hi.at(0, j), ss);
+        }
+        ss = lanes_sum<LANES>(on ? ss : 0.f, lanes);   // a slot that nothing was copied to holds anything
+        fetch(here);                                   // the sum has read this slot
+        slot = (slot + 1) & (D - 1);
+        const float n = rsqrtf(fmaf(ss, P.inv_hd, P.eps));
+        float ol[1][V], oh[1][V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xl = lo.at(0, j), xh = hi.at(0, j);
+          ol[0][j] = n * fmaf(xl, ac[0][j], -xh * as[0][j]);
+          oh[0][j] = n * fmaf(xh, bc[0][j], xl * bs[0][j]);
+        }
+        if (on) {
+          store_piece<DT, V, 1>(o, ol, 0, 1, V);
+          store_piece<DT, V, 1>(o + P.half, oh, 0, 1, V);
+        }
+        head += hstep;
+        o += ostep;
+      }
+    }
+  }
+}
+
+// The tables and weights of a step are read from shared memory, widened: in registers they would
+// take half of what a thread may have, and packed there their widening at every step measured a
+// fifth of the instructions.
+template <int DT> struct BwdShared {
+  static constexpr int kV = DT == ZT_F32 ? 4 : 8;
+  uint4 ring[kBwdWarps][kBwdRing][4][32];
+  float table[kBwdWarps][4][kV / 4][32][4];   // cos, cos', sin, sin' of the warp's position
+  float weight[2][2][kV / 4][32][4];          // of q and k, both halves
+};
+
+template <int DT, int LANES>
+__global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_backward_ring_kernel(const __grid_constant__ QkParams P) {
+  using T = typename El<DT>::T;
+  constexpr int V = 16 / (int)sizeof(T), D = kBwdRing;
+  constexpr uint32_t kSide = V * 128;   // bytes of a warp's V fp32 values a lane
+  extern __shared__ uint4 dynamic[];    // BwdShared; at the end the warps' sums
+  BwdShared<DT>& S = *reinterpret_cast<BwdShared<DT>*>(dynamic);
+  const int lanes = LANES > 0 ? LANES : P.lanes, per_warp = 32 / lanes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, sub = lane & (lanes - 1), mine = lane / lanes;
+  const uint32_t ring = smem_at(&S.ring[warp][0][0][lane]);   // a step's slot is 2048 bytes
+  const uint32_t table = smem_at(&S.table[warp][0][0][lane]), weight = smem_at(&S.weight[0][0][0][lane]);
+  const bool in = sub * V < P.half;
+  float dl[2][1][V], dh[2][1][V];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int j = 0; j < V; ++j) dl[a][0][j] = dh[a][0][j] = 0.f;
+
+  Cursor<T, true> ahead;
+  ahead.item = blockIdx.x * kBwdWarps + warp;
+  ahead.items = P.rows * P.split;
+  ahead.stride = gridDim.x * kBwdWarps;
+  ahead.enter(P, 0, per_warp, mine, sub * V);
+  auto fetch = [&](uint32_t slot) {
+    if (ahead.item < ahead.items) {
+      if (in && ahead.head < P.heads[ahead.which]) {
+        copy16(slot, ahead.x);
+        copy16(slot + 512, ahead.x + P.half);
+        copy16(slot + 1024, ahead.g);
+        copy16(slot + 1536, ahead.g + P.half);
+      }
+      ahead.advance(P, per_warp, mine, sub * V);
+    }
+    copy_commit();
+  };
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) fetch(ring + d * 2048);
+  if (warp < 4) {   // q lo, q hi, k lo, k hi
+    float w[1][V];
+    load_side<DT, V, 1>(w, P.w[warp / 2], (warp & 1) * P.half, P.w_dtype, sub, lanes, P.half);
+    smem_put(weight + warp * kSide, w[0]);
+  }
+  __syncthreads();
+  int slot = 0;
+  const int items = ahead.items, stride = ahead.stride;
+  for (int item = blockIdx.x * kBwdWarps + warp; item < items; item += stride) {
+    const Item it(P, item);
+    const int64_t trow = (int64_t)(P.per_batch ? it.row : it.t) * P.hd;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v[1][V];
+      load_side<DT, V, 1>(v, i < 2 ? P.cos : P.sin, trow + (i & 1) * P.half, P.t_dtype, sub, lanes, P.half);
+      smem_put(table + i * kSide, v[0]);
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      int grp = first_of(which ? P.groups[0] : 0, it.part, P.split);
+      if (grp >= P.groups[which]) continue;
+      const int hstep = per_warp * P.split, heads = P.heads[which];
+      int head = grp * per_warp + mine;
+      T* o = it.at(static_cast<T*>(P.out[which]), P.os[which], head) + sub * V;
+      const int64_t ostep = hstep * P.os[which][2];
+      for (; grp < P.groups[which]; grp += P.split) {
+        const bool on = in && head < heads;
+        const uint32_t here = ring + slot * 2048;
+        copy_wait<D - 1>();
+        Piece<DT, V, 1> xl, xh, gl, gh;
+        gl.take(smem_load16(here + 1024));
+        gh.take(smem_load16(here + 1536));
+        xl.take(smem_load16(here));
+        xh.take(smem_load16(here + 512));
+        float yl[V], yh[V], wl[V], wh[V];   // dy, then w dy
+        {
+          float c[V], s[V];
+          smem_get(c, table);
+          smem_get(s, table + 3 * kSide);
+#pragma unroll
+          for (int j = 0; j < V; ++j) yl[j] = fmaf(gl.at(0, j), c[j], gh.at(0, j) * s[j]);
+          smem_get(c, table + kSide);
+          smem_get(s, table + 2 * kSide);
+#pragma unroll
+          for (int j = 0; j < V; ++j) yh[j] = fmaf(gh.at(0, j), c[j], -gl.at(0, j) * s[j]);
+        }
+        smem_get(wl, weight + which * 2 * kSide);
+        smem_get(wh, weight + which * 2 * kSide + kSide);
+        float ss = 0.f, sd = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float a = xl.at(0, j), z = xh.at(0, j);
+          ss = fmaf(a, a, ss);
+          ss = fmaf(z, z, ss);
+          wl[j] *= yl[j];
+          wh[j] *= yh[j];
+          sd = fmaf(wl[j], a, sd);
+          sd = fmaf(wh[j], z, sd);
+        }
+        ss = lanes_sum<LANES>(on ? ss : 0.f, lanes);   // a slot that nothing was copied to holds anything
+        sd = lanes_sum<LANES>(on ? sd : 0.f, lanes);
+        fetch(here);                                   // the sums have read this slot
+        slot = (slot + 1) & (D - 1);
+        if (on) {
+          const float n = rsqrtf(fmaf(ss, P.inv_hd, P.eps));
+          const float m = n * n * sd * P.inv_hd;   // dx = n w dy - (x n) m
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float a = xl.at(0, j) * n, z = xh.at(0, j) * n;
+            dl[which][0][j] = fmaf(yl[j], a, dl[which][0][j]);
+            dh[which][0][j] = fmaf(yh[j], z, dh[which][0][j]);
+            wl[j] = fmaf(-a, m, n * wl[j]);
+            wh[j] = fmaf(-z, m, n * wh[j]);
+          }
+          store_piece<DT, V, 1>(o, reinterpret_cast<const float(&)[1][V]>(wl), 0, 1, V);
+          store_piece<DT, V, 1>(o + P.half, reinterpret_cast<const float(&)[1][V]>(wh), 0, 1, V);
+        }
+        head += hstep;
+        o += ostep;
+      }
+    }
+  }
+  copy_wait<0>();
+  __syncthreads();   // the rings become the warps' sums
+  block_weights<V, 1>(P, dl, dh, reinterpret_cast<float*>(dynamic), warp, lanes, sub, mine);
+}
+
+// The blocks' weight gradients, summed in a fixed order by 32 x 32 threads per 32 columns and
 // rounded to the weights' type.
 template <int DT>
-__global__ void __launch_bounds__(256) qk_weight_kernel(const float* __restrict__ partial, int32_t blocks, int32_t hd,
-                                                        typename El<DT>::T* __restrict__ dwq,
-                                                        typename El<DT>::T* __restrict__ dwk) {
-  __shared__ float part[8][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x / 32;
+__global__ void __launch_bounds__(1024) qk_weight_kernel(const float* __restrict__ partial, int32_t blocks, int32_t hd,
+                                                         typename El<DT>::T* __restrict__ dwq,
+                                                         typename El<DT>::T* __restrict__ dwk) {
+  __shared__ float part[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x / 32, col = blockIdx.x * 32 + x;
   float v = 0.f;
-  if (col < 2 * hd)
-    for (int b = y; b < blocks; b += 8) v += partial[(int64_t)b * 2 * hd + col];
-  part[y][threadIdx.x & 31] = v;
+  if (col < 2 * hd) {
+#pragma unroll 8
+    for (int b = y; b < blocks; b += 32) v += partial[(int64_t)b * 2 * hd + col];
+  }
+  part[y][x] = v;
   __syncthreads();
-  if (y == 0 && col < 2 * hd) {
-    float s = 0.f;
+  float s = part[x][y];   // warp y now sums column y of these 32
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
-    if (col < hd) dwq[col] = El<DT>::from(s);
-    else dwk[col - hd] = El<DT>::from(s);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int c = blockIdx.x * 32 + y;
+  if (x == 0 && c < 2 * hd) {
+    if (c < hd) dwq[c] = El<DT>::from(s);
+    else dwk[c - hd] = El<DT>::from(s);
   }
 }
 
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 int bwd_blocks(int64_t items) {
-  const int64_t need = (items + kBwdWarps - 1) / kBwdWarps, most = (int64_t)zt::sm_count() * 2;
+  const int64_t need = (items + kBwdWarps - 1) / kBwdWarps, most = (int64_t)zt::sm_count() * kBwdBlocks;
   return (int)(need < most ? need : most);
 }
 
-// Whether a lane can take 16 bytes at a time: the halves and every stride are whole
-// vectors and every pointer is aligned to them.
-bool wide(const zt_qk_args* a, bool backward) {
+// Whether a call's heads can go through the ring, 16 bytes a lane: whole 16-byte vectors
+// everywhere, at most 32 of them in a half. Else a lane takes single elements (head
+// sizes that are no multiple of 16 elements, 8 in fp32; views off their alignment).
+bool ring_fits(const zt_qk_args* a, bool backward) {
   const int v = a->dtype == ZT_F32 ? 4 : 8;
-  if ((a->head_dim / 2) % v) return false;
-  auto strides = [&](const int64_t* s) { return s[0] % v == 0 && s[1] % v == 0 && s[2] % v == 0; };
-  const void* ptrs[] = {a->q, a->k, a->q_out, a->k_out, a->q_weight, a->k_weight, a->cos, a->sin};
-  for (const void* p : ptrs)
+  if ((a->head_dim / 2) % v || a->head_dim / 2 > 32 * v) return false;
+  auto strides = [&](const int64_t* s) {   // those of a dimension of one are never used
+    return (a->batch == 1 || s[0] % v == 0) && (a->seq == 1 || s[1] % v == 0) &&
+           ((a->q_heads == 1 && a->k_heads == 1) || s[2] % v == 0);
+  };
+  for (const void* p : {a->q, a->k, (const void*)a->q_out, (const void*)a->k_out, a->q_weight, a->k_weight, a->cos, a->sin})
     if (!aligned(p, 16)) return false;
   if (!strides(a->q_strides) || !strides(a->k_strides) || !strides(a->q_out_strides) || !strides(a->k_out_strides))
     return false;
-  if (backward && (!aligned(a->q_grad, 16) || !aligned(a->k_grad, 16) || !strides(a->q_grad_strides) ||
-                   !strides(a->k_grad_strides)))
-    return false;
-  return true;
+  return !backward || (aligned(a->q_grad, 16) && aligned(a->k_grad, 16) && strides(a->q_grad_strides) &&
+                       strides(a->k_grad_strides));
 }
 
 int check_args(const zt_qk_args* a, bool backward, const char* who) {
@@ -424,8 +765,8 @@ int pow2_at_least(int v) {
 
 // Lanes of a head, and the warps that share a position's heads: 1 where the positions
 // alone give every SM `per_sm` warps, else as many as bring the launch up to that.
-void shape(const zt_qk_args* a, bool is_wide, int per_sm, QkParams* P) {
-  const int v = is_wide ? (a->dtype == ZT_F32 ? 4 : 8) : 1;
+void shape(const zt_qk_args* a, bool ring, int per_sm, QkParams* P) {
+  const int v = !ring ? 1 : a->dtype == ZT_F32 ? 4 : 8;
   P->hd = a->head_dim;
   P->half = a->head_dim / 2;
   const int lanes = pow2_at_least((P->half + v - 1) / v);
@@ -462,27 +803,47 @@ void fill(const zt_qk_args* a, QkParams* P) {
   }
 }
 
-template <int DT, int V, int NC, bool SAME>
-void launch_one(const QkParams& P, bool backward, int blocks, cudaStream_t s) {
+template <int DT, int LANES> int launch_ring(const QkParams& P, bool backward, int blocks, cudaStream_t s) {
+  if (!backward) {
+    qk_forward_ring_kernel<DT, LANES><<<blocks, 32 * kWarps, 0, s>>>(P);
+    return ZT_OK;
+  }
+  static std::mutex mu;
+  static bool ready[64] = {false};
+  int dev = 0;
+  if (int rc = zt::check_cuda(cudaGetDevice(&dev), "zt_qk_norm_rope_backward: cudaGetDevice")) return rc;
+  if (dev < 0 || dev >= 64) return zt::set_error(ZT_ERR_LIMIT, "zt_qk_norm_rope_backward: device ordinal >= 64");
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!ready[dev]) {
+      if (int rc = zt::check_cuda(cudaFuncSetAttribute(qk_backward_ring_kernel<DT, LANES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       (int)sizeof(BwdShared<DT>)), "zt_qk_norm_rope_backward: shared memory attribute"))
+        return rc;
+      ready[dev] = true;
+    }
+  }
+  qk_backward_ring_kernel<DT, LANES><<<blocks, 32 * kBwdWarps, sizeof(BwdShared<DT>), s>>>(P);
+  return ZT_OK;
+}
+
+template <int DT> int launch_typed(const QkParams& P, bool backward, bool ring, int blocks, cudaStream_t s) {
+  if (ring) {
+    if (P.lanes == 4) return launch_ring<DT, 4>(P, backward, blocks, s);
+    if (P.lanes == 8) return launch_ring<DT, 8>(P, backward, blocks, s);
+    if (P.lanes == 16) return launch_ring<DT, 16>(P, backward, blocks, s);
+    return launch_ring<DT, 0>(P, backward, blocks, s);
+  }
   if (backward)
-    qk_backward_kernel<DT, V, NC, SAME><<<blocks, 32 * kBwdWarps, sizeof(float) * kBwdWarps * 2 * P.hd, s>>>(P);
+    qk_backward_kernel<DT><<<blocks, 32 * kBwdWarps, sizeof(float) * kBwdWarps * 2 * P.hd, s>>>(P);
   else
-    qk_forward_kernel<DT, V, NC, SAME><<<blocks, 32 * kWarps, 0, s>>>(P);
+    qk_forward_kernel<DT><<<blocks, 32 * kWarps, 0, s>>>(P);
+  return ZT_OK;
 }
 
-template <int DT>
-void launch_half(const QkParams& P, bool backward, bool is_wide, bool same, int blocks, cudaStream_t s) {
-  if (is_wide) same ? launch_one<DT, 8, 1, true>(P, backward, blocks, s) : launch_one<DT, 8, 1, false>(P, backward, blocks, s);
-  else same ? launch_one<DT, 1, kE, true>(P, backward, blocks, s) : launch_one<DT, 1, kE, false>(P, backward, blocks, s);
-}
-
-void launch(const zt_qk_args* a, const QkParams& P, bool backward, bool is_wide, int blocks, cudaStream_t s) {
-  const bool same = a->weight_dtype == a->dtype && a->table_dtype == a->dtype;
-  if (a->dtype == ZT_BF16) return launch_half<ZT_BF16>(P, backward, is_wide, same, blocks, s);
-  if (a->dtype == ZT_F16) return launch_half<ZT_F16>(P, backward, is_wide, same, blocks, s);
-  if (!is_wide) return launch_one<ZT_F32, 1, kE, true>(P, backward, blocks, s);
-  if (P.half <= 128) return launch_one<ZT_F32, 4, 1, true>(P, backward, blocks, s);
-  launch_one<ZT_F32, 4, 2, true>(P, backward, blocks, s);
+int launch(const zt_qk_args* a, const QkParams& P, bool backward, bool ring, int blocks, cudaStream_t s) {
+  if (a->dtype == ZT_F32) return launch_typed<ZT_F32>(P, backward, ring, blocks, s);
+  if (a->dtype == ZT_BF16) return launch_typed<ZT_BF16>(P, backward, ring, blocks, s);
+  return launch_typed<ZT_F16>(P, backward, ring, blocks, s);
 }
 
 }  // namespace
@@ -494,11 +855,12 @@ int zt_qk_norm_rope(const zt_qk_args* a, void* stream) {
   if (int rc = check_args(a, false, "zt_qk_norm_rope")) return rc;
   if (a->batch * a->seq == 0) return ZT_OK;
   QkParams P = {};
-  const bool is_wide = wide(a, false);
-  shape(a, is_wide, 32, &P);
+  const bool ring = ring_fits(a, false);
+  shape(a, ring, kFwdBlocks * kWarps, &P);
   fill(a, &P);
-  const int64_t items = (int64_t)P.rows * P.split;
-  launch(a, P, false, is_wide, (int)((items + kWarps - 1) / kWarps), zt::as_stream(stream));
+  int64_t blocks = ((int64_t)P.rows * P.split + kWarps - 1) / kWarps;
+  if (ring && blocks > (int64_t)zt::sm_count() * kFwdBlocks) blocks = (int64_t)zt::sm_count() * kFwdBlocks;
+  if (int rc = launch(a, P, false, ring, (int)blocks, zt::as_stream(stream))) return rc;
   return zt::check_cuda(cudaGetLastError(), "zt_qk_norm_rope launch");
 }
 
@@ -508,7 +870,7 @@ size_t zt_qk_norm_rope_workspace_bytes(int32_t head_dim) {
     zt::set_error(ZT_ERR_INVALID, "zt_qk_norm_rope_workspace_bytes: head_dim must be even and at most 512");
     return 0;
   }
-  return sizeof(float) * 2 * (size_t)head_dim * (size_t)(zt::sm_count() * 2);
+  return sizeof(float) * 2 * (size_t)head_dim * (size_t)(zt::sm_count() * kBwdBlocks);
 }
 
 int zt_qk_norm_rope_backward(const zt_qk_args* a, void* stream) {
@@ -520,23 +882,23 @@ int zt_qk_norm_rope_backward(const zt_qk_args* a, void* stream) {
   if (a->batch * a->seq > 0) {
     if (a->workspace_bytes < zt_qk_norm_rope_workspace_bytes(a->head_dim))
       return zt::set_error(ZT_ERR_INVALID, "zt_qk_norm_rope_backward: workspace too small");
-    const bool is_wide = wide(a, true);
-    shape(a, is_wide, 2 * kBwdWarps, &P);
+    const bool ring = ring_fits(a, true);
+    shape(a, ring, kBwdBlocks * kBwdWarps, &P);
     fill(a, &P);
     blocks = bwd_blocks((int64_t)P.rows * P.split);
-    launch(a, P, true, is_wide, blocks, s);
+    if (int rc = launch(a, P, true, ring, blocks, s)) return rc;
     if (int rc = zt::check_cuda(cudaGetLastError(), "zt_qk_norm_rope_backward launch")) return rc;
   }
   const unsigned grid = (unsigned)((2 * a->head_dim + 31) / 32);
   const float* part = static_cast<const float*>(a->workspace);
   if (a->weight_dtype == ZT_F32)
-    qk_weight_kernel<ZT_F32><<<grid, 256, 0, s>>>(part, blocks, a->head_dim, static_cast<float*>(a->dq_weight),
+    qk_weight_kernel<ZT_F32><<<grid, 1024, 0, s>>>(part, blocks, a->head_dim, static_cast<float*>(a->dq_weight),
                                                   static_cast<float*>(a->dk_weight));
   else if (a->weight_dtype == ZT_BF16)
-    qk_weight_kernel<ZT_BF16><<<grid, 256, 0, s>>>(part, blocks, a->head_dim, static_cast<__nv_bfloat16*>(a->dq_weight),
+    qk_weight_kernel<ZT_BF16><<<grid, 1024, 0, s>>>(part, blocks, a->head_dim, static_cast<__nv_bfloat16*>(a->dq_weight),
                                                    static_cast<__nv_bfloat16*>(a->dk_weight));
   else
-    qk_weight_kernel<ZT_F16><<<grid, 256, 0, s>>>(part, blocks, a->head_dim, static_cast<__half*>(a->dq_weight),
+    qk_weight_kernel<ZT_F16><<<grid, 1024, 0, s>>>(part, blocks, a->head_dim, static_cast<__half*>(a->dq_weight),
                                                   static_cast<__half*>(a->dk_weight));
   return zt::check_cuda(cudaGetLastError(), "zt_qk_norm_rope_backward: weight launch");
 }

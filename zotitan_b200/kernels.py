@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -926,15 +927,31 @@ def lowrank_take_error() -> int:
 
 # ---- query / key norms with the rotary embedding -------------------------------------------
 
+# The argument structs of the entry points below as their C layout (include/zotitan_b200.h):
+# packing one costs a few hundred nanoseconds, filling a ctypes.Structure several microseconds,
+# which the smallest calls would notice.
+_QK_ARGS = struct.Struct("14Q20q7if")
+_DISTILL_ARGS = struct.Struct("9Q4q4ifi")
+_LINEAR_DISTILL_ARGS = struct.Struct("8Q3q3if2iq")
+
+
 def _on(device: torch.device):
     """The device of a call's tensors as the current one (nothing to switch in the usual case)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def _same_device(first: torch.Tensor, **others):
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _raw_stream(device: torch.device) -> int:
+    """The current stream of `device`, as _stream_ptr gives it, without building its object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _same_device(device: torch.device, **others):
     for name, t in others.items():
-        if t.device != first.device:
-            raise ValueError(f"{name} must be on {first.device}, not {t.device}")
+        if t.device != device:
+            raise ValueError(f"{name} must be on {device}, not {t.device}")
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
@@ -958,60 +975,58 @@ def _shares_memory_inside(t: torch.Tensor) -> bool:
     return False
 
 
-def _qk_strides(t: torch.Tensor):
-    return (ctypes.c_int64 * 3)(*(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())))
-
-
 def _check_qk(q, k, q_weight, k_weight, cos, sin):
-    """The operands as [batch, position, head, head_dim] views with unit stride in a head;
-    (q, k, cos, sin, whether every sequence has its own cos / sin rows)."""
-    _check_cuda(q, "q")
-    if q.dtype not in _DT:
+    """The operands as [batch, position, head, head_dim] views; (q, k, cos, sin, whether every
+    sequence has its own cos / sin rows)."""
+    device, dtype, shape, k_shape = q.device, q.dtype, q.shape, k.shape
+    if device.type != "cuda":
+        raise ValueError("q must be a CUDA tensor")
+    if dtype not in _DT:
         raise ValueError("q must be fp32, bf16 or fp16")
-    if q.dim() not in (3, 4) or k.dim() != q.dim():
+    dims = len(shape)
+    if dims not in (3, 4) or len(k_shape) != dims:
         raise ValueError("q and k must be [positions, heads, head_dim] or [batch, positions, heads, head_dim]")
-    if q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1] or k.dtype != q.dtype:
+    hd = shape[-1]
+    if shape[:-2] != k_shape[:-2] or hd != k_shape[-1] or k.dtype != dtype:
         raise ValueError("q and k must agree in positions, head_dim and dtype")
-    hd = q.shape[-1]
     if hd < 2 or hd % 2 or hd > 512:
         raise ValueError("head_dim must be even and at most 512")
-    if q.shape[-2] == 0 or k.shape[-2] == 0:
+    if shape[-2] == 0 or k_shape[-2] == 0:
         raise ValueError("q and k must have heads")
-    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if t.shape != (hd,) or t.dtype != q_weight.dtype or t.dtype not in (q.dtype, torch.float32):
-            raise ValueError(f"{name} must be a [head_dim] vector of q's dtype or fp32, both weights alike")
-    if q.dim() == 3:
+    w_dtype, t_dtype = q_weight.dtype, cos.dtype
+    if (q_weight.shape != (hd,) or k_weight.shape != (hd,) or k_weight.dtype != w_dtype
+            or (w_dtype != dtype and w_dtype != torch.float32)):
+        raise ValueError("q_weight and k_weight must be [head_dim] vectors of q's dtype or fp32, both alike")
+    if dims == 3:
         q, k = q.unsqueeze(0), k.unsqueeze(0)
-    B, T = q.shape[:2]
-    if cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in (q.dtype, torch.float32):
+        shape = q.shape
+    B, T = shape[:2]
+    table = cos.shape
+    if table != sin.shape or t_dtype != sin.dtype or (t_dtype != dtype and t_dtype != torch.float32):
         raise ValueError("cos and sin must agree and have q's dtype or fp32")
-    if cos.shape not in ((T, hd), (1, T, hd), (B, T, hd)):
+    if table != (1, T, hd) and table != (B, T, hd) and table != (T, hd):
         raise ValueError("cos and sin must be [positions, head_dim], with a leading 1 or batch")
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("cos and sin are constants: detach them")
-    _same_device(q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin)
-    own_rows = cos.dim() == 3 and cos.shape[0] != 1
-    return q, k, cos.contiguous(), sin.contiguous(), own_rows
+    if not (device == k.device == q_weight.device == k_weight.device == cos.device == sin.device):
+        _same_device(device, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin)
+    return q, k, cos.contiguous(), sin.contiguous(), len(table) == 3 and table[0] != 1
 
 
-def _qk_args(q, k, q_out, k_out, q_weight, k_weight, cos, sin, eps, own_rows):
-    a = L.ZtQkArgs()
-    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    a.q_weight, a.k_weight, a.cos, a.sin = q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr()
-    a.q_strides, a.k_strides = _qk_strides(q), _qk_strides(k)
-    a.q_out_strides, a.k_out_strides = _qk_strides(q_out), _qk_strides(k_out)
-    a.batch, a.seq, a.q_heads, a.head_dim = q.shape
-    a.k_heads = k.shape[2]
-    a.dtype, a.weight_dtype, a.table_dtype = _DT[q.dtype], _DT[q_weight.dtype], _DT[cos.dtype]
-    a.table_batch, a.eps = int(own_rows), eps
-    return a
-
-
-def _qk_forward(q, k, q_weight, k_weight, cos, sin, eps, own_rows, q_out, k_out):
-    a = _qk_args(q, k, q_out, k_out, q_weight, k_weight, cos, sin, eps, own_rows)
-    with _on(q.device):
-        L.check(L.load().zt_qk_norm_rope(ctypes.byref(a), _stream_ptr(q.device)), "zt_qk_norm_rope")
-    return q_out, k_out
+def _qk_call(entry, q, k, q_out, k_out, q_weight, k_weight, cos, sin, eps, own_rows, gq=None, gk=None, dwq=0, dwk=0, ws=0,
+             ws_bytes=0):
+    """One call of zt_qk_norm_rope or its backward on [batch, position, head, head_dim] views."""
+    B, T, hq, hd = q.shape
+    device = q.device
+    none = (0, 0, 0)
+    args = _QK_ARGS.pack(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+                         gq.data_ptr() if gq is not None else 0, gk.data_ptr() if gk is not None else 0,
+                         q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), dwq, dwk, ws, ws_bytes,
+                         *q.stride()[:3], *k.stride()[:3], *q_out.stride()[:3], *k_out.stride()[:3],
+                         *(gq.stride()[:3] if gq is not None else none), *(gk.stride()[:3] if gk is not None else none),
+                         B, T, hq, k.shape[2], hd, _DT[q.dtype], _DT[q_weight.dtype], _DT[cos.dtype], own_rows, eps)
+    with _on(device):
+        L.check(getattr(L.load(), entry)(args, _raw_stream(device)), entry)
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
@@ -1021,35 +1036,35 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps, own_rows):
+        q, k, q_weight, k_weight = _unit(q), _unit(k), q_weight.contiguous(), k_weight.contiguous()
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
-        ctx.eps, ctx.own_rows = eps, own_rows
-        qu, ku = _unit(q), _unit(k)
-        return _qk_forward(qu, ku, q_weight.contiguous(), k_weight.contiguous(), cos, sin, eps, own_rows,
-                           torch.empty(q.shape, dtype=q.dtype, device=q.device),
-                           torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        ctx.rest = eps, own_rows
+        qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
+        _qk_call("zt_qk_norm_rope", q, k, qo, ko, q_weight, k_weight, cos, sin, eps, own_rows)
+        return qo, ko
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, cos, sin = ctx.saved_tensors
-        q, k, gq, gk = _unit(q), _unit(k), _unit(gq), _unit(gk)
-        wq, wk = q_weight.contiguous(), k_weight.contiguous()
-        dev = q.device
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        dw = torch.empty((2, q.shape[-1]), dtype=wq.dtype, device=dev)
-        lib = L.load()
-        with _on(dev):
-            ws = torch.empty(lib.zt_qk_norm_rope_workspace_bytes(q.shape[-1]), dtype=torch.uint8, device=dev)
-            a = _qk_args(q, k, dq, dk, wq, wk, cos, sin, ctx.eps, ctx.own_rows)
-            a.q_grad, a.k_grad, a.q_grad_strides, a.k_grad_strides = (gq.data_ptr(), gk.data_ptr(), _qk_strides(gq),
-                                                                      _qk_strides(gk))
-            a.dq_weight, a.dk_weight = dw[0].data_ptr(), dw[1].data_ptr()
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-            L.check(lib.zt_qk_norm_rope_backward(ctypes.byref(a), _stream_ptr(dev)), "zt_qk_norm_rope_backward")
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dw[0] if need[2] else None,
-                dw[1] if need[3] else None, None, None, None, None)
+        return (_qk_backward_once if torch.is_grad_enabled() else _qk_backward)(ctx, gq, gk)
+
+
+def _qk_backward(ctx, gq, gk):
+    q, k, wq, wk, cos, sin = ctx.saved_tensors
+    gq, gk = _unit(gq), _unit(gk)
+    hd = q.shape[-1]
+    dq, dk, dw = q.new_empty(q.shape), k.new_empty(k.shape), wq.new_empty((2, hd))
+    with _on(q.device):
+        ws = q.new_empty(L.load().zt_qk_norm_rope_workspace_bytes(hd), dtype=torch.uint8)
+    at = dw.data_ptr()
+    _qk_call("zt_qk_norm_rope_backward", q, k, dq, dk, wq, wk, cos, sin, *ctx.rest, gq, gk, at, at + hd * dw.element_size(),
+             ws.data_ptr(), ws.numel())
+    need = ctx.needs_input_grad
+    return (dq if need[0] else None, dk if need[1] else None, dw[0] if need[2] else None, dw[1] if need[3] else None,
+            None, None, None, None)
+
+
+# with create_graph=True: the same values, and an error where they are differentiated again
+_qk_backward_once = torch.autograd.function.once_differentiable(_qk_backward)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
@@ -1059,16 +1074,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     head_dim] (an optional leading batch; any strides, a fused projection's slices among
     them), norm weights [head_dim], cos and sin [positions, head_dim], [1, ...] or [batch, ...]
     (the halves of a head rotate against each other). fp32 inside, one rounding: returns new
-    contiguous (q, k). Differentiable in q, k and the weights (sums in a fixed order)."""
+    contiguous (q, k). Differentiable once in q, k and the weights (sums in a fixed order)."""
     q4, k4, cos, sin, own_rows = _check_qk(q, k, q_weight, k_weight, cos, sin)
     eps = float(eps)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
         qo, ko = _QkNormRope.apply(q4, k4, q_weight, k_weight, cos, sin, eps, own_rows)
     else:
         q4, k4 = _unit(q4), _unit(k4)
-        qo, ko = _qk_forward(q4, k4, q_weight.contiguous(), k_weight.contiguous(), cos, sin, eps, own_rows,
-                             torch.empty(q4.shape, dtype=q.dtype, device=q.device),
-                             torch.empty(k4.shape, dtype=k.dtype, device=q.device))
+        qo, ko = q4.new_empty(q4.shape), k4.new_empty(k4.shape)
+        _qk_call("zt_qk_norm_rope", q4, k4, qo, ko, q_weight.contiguous(), k_weight.contiguous(), cos, sin, eps, own_rows)
     return (qo, ko) if q.dim() == 4 else (qo[0], ko[0])
 
 
@@ -1084,6 +1098,8 @@ def qk_norm_rope_(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
             raise ValueError(f"{name} must have unit stride inside a head")
         if _shares_memory_inside(t):
             raise ValueError(f"{name} names the same element twice (an expanded view)")
+        if any(_overlap(t, o) for o in (q_weight, k_weight, cos, sin)):
+            raise ValueError(f"{name} overlaps a weight or a table")
     if _overlap(q4, k4):
         # slices of the same rows: equal position strides, disjoint inside a position
         rows = [(d, q4.stride(d)) for d in (0, 1) if q4.shape[d] > 1]
@@ -1094,37 +1110,42 @@ def qk_norm_rope_(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
     for t in (q, k):
         if not t.is_inference():
             torch.autograd.graph.increment_version(t)
-    _qk_forward(q4, k4, q_weight.contiguous(), k_weight.contiguous(), cos, sin, float(eps), own_rows, q4, k4)
+    _qk_call("zt_qk_norm_rope", q4, k4, q4, k4, q_weight.contiguous(), k_weight.contiguous(), cos, sin, float(eps), own_rows)
     return q, k
 
 
 # ---- distillation from a teacher's top logits ----------------------------------------------
 
-def _check_list(rows: int, like: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.Tensor, temperature: float):
-    if top_idx.dim() != 2 or top_idx.shape[0] != rows or top_idx.dtype not in (torch.int32, torch.int64):
+def _check_list(rows: int, device, top_idx: torch.Tensor, top_logits: torch.Tensor, temperature: float):
+    shape = top_idx.shape
+    if len(shape) != 2 or shape[0] != rows or top_idx.dtype not in (torch.int64, torch.int32):
         raise ValueError("top_idx must be an int32 or int64 [rows, top] matrix")
-    if top_logits.shape != top_idx.shape or top_logits.dtype not in _DT:
+    if top_logits.shape != shape or top_logits.dtype not in _DT:
         raise ValueError("top_logits must be an fp32, bf16 or fp16 matrix of top_idx's shape")
-    if not 1 <= top_idx.shape[1] <= L.ZT_DISTILL_MAX_TOP:
+    if not 1 <= shape[1] <= L.ZT_DISTILL_MAX_TOP:
         raise ValueError(f"a teacher's list must have 1 to {L.ZT_DISTILL_MAX_TOP} entries")
     if top_logits.requires_grad:
         raise ValueError("the teacher's logits are constants: detach them")
     if not 1e-3 <= temperature <= 1e3:
         raise ValueError("temperature must lie in [0.001, 1000]")
-    _same_device(like, top_idx=top_idx, top_logits=top_logits)
+    if not (device == top_idx.device == top_logits.device):
+        _same_device(device, top_idx=top_idx, top_logits=top_logits)
     return top_idx.contiguous(), top_logits.contiguous()
 
 
-def _check_logits(logits: torch.Tensor) -> torch.Tensor:
-    _check_cuda(logits, "logits")
+def _check_logits(logits: torch.Tensor) -> torch.device:
+    device = logits.device
+    if device.type != "cuda":
+        raise ValueError("logits must be a CUDA tensor")
     if logits.dtype not in _DT or logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError("logits must be an fp32, bf16 or fp16 [rows, vocab] matrix")
-    return logits
+    return device
 
 
 def _rows_of(logits: torch.Tensor) -> torch.Tensor:
     """logits with unit column stride and rows that do not overlap (a copy where they do)."""
-    if (logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+    (rows, vocab), (ld, col) = logits.shape, logits.stride()
+    if (vocab > 1 and col != 1) or (rows > 1 and ld < vocab):
         return logits.contiguous()
     return logits
 
@@ -1133,20 +1154,16 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])
 
 
-def _distill_args(logits, top_idx, top_logits, temperature):
-    a = L.ZtDistillArgs()
-    a.logits, a.top_idx, a.top_logits = logits.data_ptr(), top_idx.data_ptr(), top_logits.data_ptr()
-    a.rows, a.vocab = logits.shape
-    a.ld = _ld(logits)
-    a.dtype, a.top, a.idx_bits = _DT[logits.dtype], top_idx.shape[1], 64 if top_idx.dtype == torch.int64 else 32
-    a.top_dtype, a.temperature = _DT[top_logits.dtype], temperature
-    return a
-
-
-def _distill_out(rows: int, device, stats: bool):
-    """loss, lse [rows] and the backward's [rows, 2], views of one allocation."""
-    buf = torch.empty((4 if stats else 2) * rows, dtype=torch.float32, device=device)
-    return buf[:rows], buf[rows:2 * rows], buf[2 * rows:] if stats else None
+def _distill_call(entry, x, top_idx, top_logits, temperature, grad=None, weight=None, weight_lse=None, loss=0, lse=0, stats=0):
+    rows, vocab = x.shape
+    device = x.device
+    args = _DISTILL_ARGS.pack(x.data_ptr(), grad.data_ptr() if grad is not None else 0, top_idx.data_ptr(),
+                              top_logits.data_ptr(), weight.data_ptr() if weight is not None else 0,
+                              weight_lse.data_ptr() if weight_lse is not None else 0, loss, lse, stats, rows, vocab, _ld(x),
+                              _ld(grad) if grad is not None else 0, _DT[x.dtype], top_idx.shape[1],
+                              64 if top_idx.dtype == torch.int64 else 32, _DT[top_logits.dtype], temperature, 0)
+    with _on(device):
+        L.check(getattr(L.load(), entry)(args, _raw_stream(device)), entry)
 
 
 class _DistillRows(torch.autograd.Function):
@@ -1154,35 +1171,33 @@ class _DistillRows(torch.autograd.Function):
     def forward(ctx, logits, top_idx, top_logits, temperature):
         ctx.set_materialize_grads(False)
         x = _rows_of(logits)
-        loss = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-        lse = torch.empty_like(loss)
-        stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
-        a = _distill_args(x, top_idx, top_logits, temperature)
-        a.loss, a.lse, a.stats = loss.data_ptr(), lse.data_ptr(), stats.data_ptr()
-        with _on(x.device):
-            L.check(L.load().zt_distill_rows(ctypes.byref(a), _stream_ptr(x.device)), "zt_distill_rows")
-        ctx.save_for_backward(logits, top_idx, top_logits, stats)
+        rows = x.shape[0]
+        loss, lse = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+        stats = x.new_empty((rows, 2), dtype=torch.float32)
+        _distill_call("zt_distill_rows", x, top_idx, top_logits, temperature, loss=loss.data_ptr(), lse=lse.data_ptr(),
+                      stats=stats.data_ptr())
+        ctx.save_for_backward(x, top_idx, top_logits, stats)
         ctx.temperature = temperature
         return loss, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g, g_lse):
-        logits, top_idx, top_logits, stats = ctx.saved_tensors
-        if g is None and g_lse is None:
-            return None, None, None, None
-        x = _rows_of(logits)
-        # the logits' own row stride: rows keep their alignment
-        grad = torch.empty_strided(x.shape, (_ld(x), 1), dtype=x.dtype, device=x.device)
-        g = g.contiguous() if g is not None else None
-        g_lse = g_lse.contiguous() if g_lse is not None else None
-        a = _distill_args(x, top_idx, top_logits, ctx.temperature)
-        a.grad, a.ld_grad, a.stats = grad.data_ptr(), _ld(grad), stats.data_ptr()
-        a.weight = g.data_ptr() if g is not None else None
-        a.weight_lse = g_lse.data_ptr() if g_lse is not None else None
-        with _on(x.device):
-            L.check(L.load().zt_distill_rows_backward(ctypes.byref(a), _stream_ptr(x.device)), "zt_distill_rows_backward")
-        return grad, None, None, None
+        return (_distill_backward_once if torch.is_grad_enabled() else _distill_backward)(ctx, g, g_lse)
+
+
+def _distill_backward(ctx, g, g_lse):
+    if g is None and g_lse is None:
+        return None, None, None, None
+    x, top_idx, top_logits, stats = ctx.saved_tensors
+    # the logits' own row stride: rows keep their alignment
+    grad = x.new_empty_strided(x.shape, (_ld(x), 1))
+    _distill_call("zt_distill_rows_backward", x, top_idx, top_logits, ctx.temperature, grad=grad,
+                  weight=g.contiguous() if g is not None else None,
+                  weight_lse=g_lse.contiguous() if g_lse is not None else None, stats=stats.data_ptr())
+    return grad, None, None, None
+
+
+_distill_backward_once = torch.autograd.function.once_differentiable(_distill_backward)
 
 
 def distill_rows(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.Tensor, temperature: float = 1.0):
@@ -1192,20 +1207,18 @@ def distill_rows(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.
     With T the temperature, q = softmax(logits / T) and p = softmax(top_logits / T) over the
     list, returns (loss, lse) fp32 [rows]:
       loss = T^2 sum_k p_k (log p_k - log q[top_idx_k]),  lse = logsumexp(logits / T),
-    both 0 on rows without an entry and differentiable in the logits. An index >= vocab makes
-    its row NaN."""
-    _check_logits(logits)
+    both 0 on rows without an entry and differentiable (once) in the logits. An index >= vocab
+    makes its row NaN."""
+    device = _check_logits(logits)
     temperature = float(temperature)
-    top_idx, top_logits = _check_list(logits.shape[0], logits, top_idx, top_logits, temperature)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    top_idx, top_logits = _check_list(logits.shape[0], device, top_idx, top_logits, temperature)
+    if logits.requires_grad and torch.is_grad_enabled():
         return _DistillRows.apply(logits, top_idx, top_logits, temperature)
     x = _rows_of(logits)
-    loss, lse, _ = _distill_out(x.shape[0], x.device, False)
-    a = _distill_args(x, top_idx, top_logits, temperature)
-    a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
-    with _on(x.device):
-        L.check(L.load().zt_distill_rows(ctypes.byref(a), _stream_ptr(x.device)), "zt_distill_rows")
-    return loss, lse
+    out = x.new_empty((2, x.shape[0]), dtype=torch.float32)
+    at = out.data_ptr()
+    _distill_call("zt_distill_rows", x, top_idx, top_logits, temperature, loss=at, lse=at + 4 * x.shape[0])
+    return out[0], out[1]
 
 
 def distill_rows_grad(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.Tensor, weight: torch.Tensor,
@@ -1214,17 +1227,19 @@ def distill_rows_grad(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: t
     (zt_distill_rows_grad): returns (loss, lse, grad) with grad[r] = weight[r] dloss_r/dlogits_r
     in the logits' dtype, weight fp32 [rows]. out: where the gradient goes, `logits` itself
     included (then they are gone). Not recorded by autograd."""
-    _check_logits(logits)
+    device = _check_logits(logits)
     temperature = float(temperature)
-    top_idx, top_logits = _check_list(logits.shape[0], logits, top_idx, top_logits, temperature)
-    if weight.dtype != torch.float32 or weight.shape != (logits.shape[0],):
+    rows = logits.shape[0]
+    top_idx, top_logits = _check_list(rows, device, top_idx, top_logits, temperature)
+    if weight.dtype != torch.float32 or weight.shape != (rows,):
         raise ValueError("weight must be an fp32 [rows] vector")
-    _same_device(logits, weight=weight)
+    if weight.device != device:
+        _same_device(device, weight=weight)
     x = _rows_of(logits)
     if out is None:
-        out = torch.empty_strided(x.shape, (_ld(x), 1), dtype=x.dtype, device=x.device)
+        out = x.new_empty_strided(x.shape, (_ld(x), 1))
     else:
-        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != device:
             raise ValueError("out must have the logits' shape, dtype and device")
         if _rows_of(out) is not out:
             raise ValueError("out must have unit column stride and rows that do not overlap")
@@ -1236,14 +1251,11 @@ def distill_rows_grad(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: t
             raise ValueError("out overlaps the teacher's lists or the weights")
         if not out.is_inference():
             torch.autograd.graph.increment_version(out)
-    weight = weight.contiguous()
-    loss, lse, stats = _distill_out(x.shape[0], x.device, True)
-    a = _distill_args(x, top_idx, top_logits, temperature)
-    a.loss, a.lse, a.stats, a.weight = loss.data_ptr(), lse.data_ptr(), stats.data_ptr(), weight.data_ptr()
-    a.grad, a.ld_grad = out.data_ptr(), _ld(out)
-    with _on(x.device):
-        L.check(L.load().zt_distill_rows_grad(ctypes.byref(a), _stream_ptr(x.device)), "zt_distill_rows_grad")
-    return loss, lse, out
+    buf = x.new_empty((4, rows), dtype=torch.float32)   # loss, lse and what a row's two passes share
+    at = buf.data_ptr()
+    _distill_call("zt_distill_rows_grad", x, top_idx, top_logits, temperature, grad=out, weight=weight.contiguous(), loss=at,
+                  lse=at + 4 * rows, stats=at + 8 * rows)
+    return buf[0], buf[1], out
 
 
 def linear_distill(x: torch.Tensor, w: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.Tensor,
@@ -1254,28 +1266,30 @@ def linear_distill(x: torch.Tensor, w: torch.Tensor, top_idx: torch.Tensor, top_
     test_stall_loads / test_wait_cycles: the GEMM loads nothing and reports an expired wait."""
     if not linear_xent_supported(x, w):
         raise ValueError("x and w must be contiguous 16-byte aligned bf16 CUDA matrices with k % 64 == 0")
-    if w.shape[0] == 0 or x.shape[1] == 0:
+    (rows, k), vocab, device = x.shape, w.shape[0], x.device
+    if vocab == 0 or k == 0:
         raise ValueError("x and w must not be empty")
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         raise ValueError("linear_distill is forward only: use distill_rows on the logits, or losses.head_distill")
     temperature = float(temperature)
-    top_idx, top_logits = _check_list(x.shape[0], x, top_idx, top_logits, temperature)
-    _same_device(x, w=w)
-    rows, k = x.shape
-    dev = x.device
+    top_idx, top_logits = _check_list(rows, device, top_idx, top_logits, temperature)
+    if w.device != device:
+        _same_device(device, w=w)
     lib = L.load()
-    with _on(dev):
-        need = lib.zt_linear_distill_workspace_bytes(rows, w.shape[0], k, top_idx.shape[1])
+    top = top_idx.shape[1]
+    with _on(device):
+        need = lib.zt_linear_distill_workspace_bytes(rows, vocab, k, top)
         if need == 0:
             L.check(L.ZT_ERR_INVALID, "zt_linear_distill_workspace_bytes")
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        loss, lse, _ = _distill_out(rows, dev, False)
-        a = L.ZtLinearDistillArgs(x.data_ptr(), w.data_ptr(), top_idx.data_ptr(), top_logits.data_ptr(), loss.data_ptr(),
-                                  lse.data_ptr(), ws.data_ptr(), need, rows, w.shape[0], k, top_idx.shape[1],
-                                  64 if top_idx.dtype == torch.int64 else 32, _DT[top_logits.dtype], temperature,
-                                  int(test_stall_loads), 0, int(test_wait_cycles))
-        L.check(lib.zt_linear_distill(ctypes.byref(a), _stream_ptr(dev)), "zt_linear_distill")
-    return loss, lse
+        ws = x.new_empty(need, dtype=torch.uint8)
+        out = x.new_empty((2, rows), dtype=torch.float32)
+        at = out.data_ptr()
+        args = _LINEAR_DISTILL_ARGS.pack(x.data_ptr(), w.data_ptr(), top_idx.data_ptr(), top_logits.data_ptr(), at,
+                                         at + 4 * rows, ws.data_ptr(), need, rows, vocab, k, top,
+                                         64 if top_idx.dtype == torch.int64 else 32, _DT[top_logits.dtype], temperature,
+                                         int(test_stall_loads), 0, int(test_wait_cycles))
+        L.check(lib.zt_linear_distill(args, _raw_stream(device)), "zt_linear_distill")
+    return out[0], out[1]
 
 
 def linear_distill_take_error() -> int:
