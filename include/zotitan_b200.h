@@ -614,7 +614,7 @@ typedef struct zt_distill_args {
   const float* weight_lse; /* [rows] gradient of lse, or NULL (backward, grad) */
   float* loss;             /* [rows] out (rows, grad) */
   float* lse;              /* [rows] out (rows, grad) */
-  float* stats;            /* [rows, 2] out (rows: may be NULL; grad), in (backward): what the backward needs */
+  float* stats;            /* [rows, 2] out (rows, grad: may be NULL), in (backward): what the backward needs */
   int64_t rows, vocab, ld, ld_grad;
   int32_t dtype;           /* ZT_F32, ZT_BF16 or ZT_F16 */
   int32_t top;             /* 1 .. ZT_DISTILL_MAX_TOP */
@@ -631,7 +631,7 @@ ZT_API int zt_distill_rows(const zt_distill_args* args, void* stream);
  * logits, lists and temperature and the stats of zt_distill_rows. */
 ZT_API int zt_distill_rows_backward(const zt_distill_args* args, void* stream);
 
-/* Both at once, for weights known beforehand: loss, lse, stats and
+/* Both at once, for weights known beforehand: loss, lse and
  * grad[r, :] = weight[r] d loss_r / dz_r (+ weight_lse[r] d lse_r / dz_r). */
 ZT_API int zt_distill_rows_grad(const zt_distill_args* args, void* stream);
 

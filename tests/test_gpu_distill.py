@@ -248,7 +248,14 @@ def test_rows_that_are_not_numbers():
     """NaN and infinities stay in their rows, and rows without a teacher take none of them."""
     from zotitan_b200 import kernels as K
     z, idx, val = make(10, 5001, 12, torch.float32, seed=6, empty=False)
-    clean = K.distill_rows_grad(z, idx, val, torch.ones(10, device="cuda"))
+    ones = torch.ones(10, device="cuda")
+
+    def both_ways():   # each entry point adds a row up in its own order
+        leaf = z.detach().clone().requires_grad_()
+        loss, lse = K.distill_rows(leaf, idx, val)
+        return (loss.detach(), lse.detach(), *torch.autograd.grad(loss, leaf, ones)), K.distill_rows_grad(z, idx, val, ones)
+
+    clean = both_ways()
     z[0, 4000] = math.nan
     z[1, 7] = math.inf
     z[2] = -math.inf
@@ -260,11 +267,7 @@ def test_rows_that_are_not_numbers():
     idx[7] = -1                                       # no teacher: whatever the logits are
     z[8, 3], idx[8, 1:], val[8, 1:] = math.inf, -5, math.nan
     val[8, 0] = -math.inf                             # no teacher either
-    leaf = z.detach().requires_grad_()
-    loss, lse = K.distill_rows(leaf, idx, val)
-    grad, = torch.autograd.grad(loss, leaf, torch.ones(10, device="cuda"))
-    one = K.distill_rows_grad(z, idx, val, torch.ones(10, device="cuda"))
-    for lo, ls, gr in ((loss, lse, grad), one):
+    for (lo, ls, gr), was in zip(both_ways(), clean):
         assert torch.isnan(lo[:6]).all() and lo[6] == math.inf
         for r in (0, 1, 2, 3):
             assert torch.isnan(ls[r]) and torch.isnan(gr[r]).all()
@@ -272,7 +275,7 @@ def test_rows_that_are_not_numbers():
             assert torch.isnan(gr[r]).any()
         for r in (7, 8):
             assert lo[r] == 0 and ls[r] == 0 and not gr[r].any()
-        assert torch.equal(lo[9], clean[0][9]) and torch.equal(gr[9], clean[2][9])
+        assert torch.equal(lo[9], was[0][9]) and torch.equal(gr[9], was[2][9])
         assert torch.isfinite(gr[6]).all()
 
 

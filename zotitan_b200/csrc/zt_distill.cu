@@ -6,13 +6,12 @@
 //   d loss / dz_v = T (q_v - sum over k with i_k = v of p_k),  d lse / dz_v = q_v / T
 //
 // Bandwidth is the bound: the forward reads each logit once, the backward reads it and
-// writes its gradient, and zt_distill_rows_grad, whose row weights are known beforehand,
-// holds the row in the shared memory of a CTA cluster and so reads and writes once in all.
-// One more warp than those that stream the row reads the teacher's list, gathers the listed
-// logits and does the list's arithmetic while the row passes by.
+// writes its gradient, and zt_distill_rows_grad, whose row weights are known beforehand, does
+// both while the row is still in L2, so that memory is read and written once in all.
+// A CTA takes a row, or with few rows a cluster of CTAs does, merging their sums over
+// distributed shared memory. One more warp than those that stream the row reads the teacher's
+// list, gathers the listed logits and does the list's arithmetic while the row passes by.
 #include <math.h>
-
-#include <mutex>
 
 #include "zt_distill.cuh"
 #include "zt_tc.cuh"
@@ -24,9 +23,12 @@ using zt::tc::cluster_rank;
 using zt::tc::cluster_sync_all;
 using zt::tc::peer_addr;
 
-constexpr int kStream = 256;             // threads that stream the row
-constexpr int kThreads = kStream + 32;   // and the list's warp
-constexpr int kWarps = kStream / 32;
+// Threads that stream a row, beside the list's warp, and the CTAs of an SM. A thread's step is two
+// vectors in the forward and four elsewhere. The forward lives on warps: of 4096 x 128256 bf16 it
+// takes 180 us with six CTAs of two vectors, 184 with four of four, 199 to 226 where
+// a thread also loads its next step ahead (its registers cost warps).
+constexpr int kSumThreads = 256, kSumCtas = 6, kSumStep = 2;
+constexpr int kWriteThreads = 512, kWriteCtas = 2, kWriteStep = 4;   // backward, and loss and gradient at once
 constexpr int kMaxCluster = 8;
 
 struct RowsParams {
@@ -52,6 +54,16 @@ template <> struct El<ZT_F32> {
   static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
     f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
   }
+  template <int U> static __device__ __forceinline__ float max_of(const uint4 (&u)[U]) {   // NaN aside
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float f[4];
+      unpack(u[i], f);
+      m = fmaxf(m, fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])));
+    }
+    return m;
+  }
   static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
@@ -68,6 +80,15 @@ template <> struct El<ZT_BF16> {
       f[2 * i] = __uint_as_float(w[i] << 16);
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
+  }
+  template <int U> static __device__ __forceinline__ float max_of(const uint4 (&u)[U]) {   // NaN aside, two at a time
+    using P2 = __nv_bfloat162;
+    auto two = [](const uint32_t& w) { return *reinterpret_cast<const P2*>(&w); };
+    P2 m = __hmax2(__hmax2(two(u[0].x), two(u[0].y)), __hmax2(two(u[0].z), two(u[0].w)));
+#pragma unroll
+    for (int i = 1; i < U; ++i)
+      m = __hmax2(m, __hmax2(__hmax2(two(u[i].x), two(u[i].y)), __hmax2(two(u[i].z), two(u[i].w))));
+    return fmaxf(__bfloat162float(__low2bfloat16(m)), __bfloat162float(__high2bfloat16(m)));
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
     uint32_t w[4];
@@ -92,6 +113,15 @@ template <> struct El<ZT_F16> {
       f[2 * i] = v.x;
       f[2 * i + 1] = v.y;
     }
+  }
+  template <int U> static __device__ __forceinline__ float max_of(const uint4 (&u)[U]) {   // NaN aside, two at a time
+    using P2 = __half2;
+    auto two = [](const uint32_t& w) { return *reinterpret_cast<const P2*>(&w); };
+    P2 m = __hmax2(__hmax2(two(u[0].x), two(u[0].y)), __hmax2(two(u[0].z), two(u[0].w)));
+#pragma unroll
+    for (int i = 1; i < U; ++i)
+      m = __hmax2(m, __hmax2(__hmax2(two(u[i].x), two(u[i].y)), __hmax2(two(u[i].z), two(u[i].w))));
+    return fmaxf(__half2float(__low2half(m)), __half2float(__high2half(m)));
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
     uint32_t w[4];
@@ -126,16 +156,57 @@ template <int DT> __device__ __forceinline__ Span<DT> span_of(const RowsParams& 
   return Span<DT>(static_cast<const typename El<DT>::T*>(base) + row * ld, lo, hi);
 }
 
-// The block's (m, s): the stream warps' in warp order. All stream threads call it.
-__device__ __forceinline__ void block_stat(Stat st, float c, Stat* red) {
-  st = warp_merge(st, c);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = st;
+// Step g of S threads, U vectors each, over a span; 2^((-inf - m) c) = 0 stands in for what is beyond.
+template <int DT, int S, int U> __device__ __forceinline__ void load_step(uint4 (&u)[U], const Span<DT>& sp, int g, bool again) {
+  const uint4* v = sp.vec();
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    const int i = threadIdx.x + (g * U + j) * S;
+    if (i < sp.n_vec) {
+      u[j] = again ? __ldcg(v + i) : __ldcs(v + i);
+    } else {
+      const uint32_t w = DT == ZT_F32 ? 0xff800000u : DT == ZT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+      u[j] = make_uint4(w, w, w, w);
+    }
+  }
 }
 
-__device__ __forceinline__ Stat total_of(const Stat* red, int n, float c) {
-  Stat r = red[0];
-  for (int i = 1; i < n; ++i) r = merge(r, red[i], c);
-  return r;
+template <int DT, int S, int U> __device__ __forceinline__ int steps_of(const Span<DT>& sp) { return (sp.n_vec + U * S - 1) / (U * S); }
+
+template <int DT, int U> __device__ __forceinline__ void absorb_step(Stat& st, const uint4 (&u)[U], float c) {
+  constexpr int V = El<DT>::kVec;
+  float f[U * V];
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    float g[V];
+    El<DT>::unpack(u[j], g);
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[j * V + k] = g[k];
+  }
+  absorb(st, f, El<DT>::max_of(u), c);
+}
+
+// A thread's share of a span's sum; gives up once the row is known to have no teacher. `again`:
+// the span will be read once more and should stay in L2.
+template <int DT, int S, int U>
+__device__ __forceinline__ Stat sum_span(const Span<DT>& sp, float c, const volatile int* none, bool again) {
+  Stat st{-INFINITY, 0.f};
+  const int n = steps_of<DT, S, U>(sp), tid = threadIdx.x;
+  uint4 u[U];
+  for (int g = 0; g < n; ++g) {
+    load_step<DT, S, U>(u, sp, g, again);
+    if (*none) break;
+    absorb_step<DT, U>(st, u, c);
+  }
+  if (tid < sp.body - sp.lo) {
+    const float f[1] = {El<DT>::to(sp.row[sp.lo + tid])};
+    absorb(st, f, c);
+  }
+  if (tid < sp.hi - sp.tail()) {
+    const float f[1] = {El<DT>::to(sp.row[sp.tail() + tid])};
+    absorb(st, f, c);
+  }
+  return st;
 }
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
@@ -144,17 +215,47 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-// The parts' (m, s) of a row, merged in part order by every CTA of its cluster alike. `mine`
-// is this CTA's, in shared memory; ends with all of them read.
-__device__ __forceinline__ Stat cluster_stat(const Stat* mine, int parts, float c) {
-  cluster_sync_all();
-  Stat r{-INFINITY, 0.f};
-  for (int i = 0; i < parts; ++i) {
-    const uint32_t a = peer_addr(mine, (uint32_t)i);
-    const Stat o{ld_cluster_f32(a), ld_cluster_f32(a + 4)};
-    r = merge(r, o, c);
+// What the CTAs of a row share, and a CTA's threads.
+template <int S> struct Shared {
+  List list;
+  Stat red[S / 32];   // the warps' sums
+  Stat mine, total;   // this CTA's, the row's
+  int none, bad;      // no teacher: the row's logits need not be read; an index that does not exist
+};
+
+// The list's warp: the row's finished sum from the stream warps' and, over the cluster, the
+// parts'. Every CTA of a cluster merges alike. The block is in step before and after.
+template <int S> __device__ __forceinline__ void finish_sum(Shared<S>& sh, int parts, float c) {
+  const int lane = threadIdx.x & 31;
+  const bool list_warp = threadIdx.x >= S;
+  __syncthreads();
+  if (list_warp) {
+    Stat st = lane < S / 32 ? sh.red[lane] : Stat{-INFINITY, 0.f};
+    st = warp_merge(st, c);
+    if (lane == 0) sh.mine = st;
+    __syncwarp();
   }
-  return r;
+  if (parts > 1) {
+    cluster_sync_all();
+    if (list_warp) {
+      Stat st{-INFINITY, 0.f};
+      if (lane < parts) {
+        const uint32_t a = peer_addr(&sh.mine, (uint32_t)lane);
+        st = Stat{ld_cluster_f32(a), ld_cluster_f32(a + 4)};
+      }
+      st = warp_merge(st, c);
+      if (lane == 0) sh.total = st;
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // the peers' sums are read
+  } else if (list_warp && lane == 0) {
+    sh.total = sh.mine;
+  }
+  __syncthreads();
+}
+
+// No CTA leaves while a peer may still read its sum.
+__device__ __forceinline__ void leave(int parts) {
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // (m, s) of a row's finished sum as it is kept: no finite logit, or an index that does not
@@ -174,82 +275,48 @@ __device__ __forceinline__ void gather(List& s, const typename El<DT>::T* row, i
   }
 }
 
+// The list's warp before the sum is there: reads the list, gathers its logits in [lo, hi), and
+// the teacher's probabilities.
+template <int DT, int S>
+__device__ __forceinline__ void prepare_list(Shared<S>& sh, const RowsParams& P, int64_t row, int32_t lo, int32_t hi) {
+  const Teacher t = read_list(sh.list, P.list, row);
+  if ((threadIdx.x & 31) == 0) {
+    sh.bad = t.bad;
+    if (!t.any) *(volatile int*)&sh.none = 1;
+  }
+  gather<DT>(sh.list, static_cast<const typename El<DT>::T*>(P.z) + row * P.ld, P.list.top, lo, hi);
+  list_softmax(sh.list, P.list.top, P.c);
+}
+
+// and after: loss, lse and what the backward needs.
+template <int S> __device__ __forceinline__ void write_loss(const Shared<S>& sh, const RowsParams& P, int64_t row, Stat st) {
+  const float loss = list_loss(sh.list, P.list.top, st, P.c, P.temperature);
+  if ((threadIdx.x & 31) == 0) {
+    P.loss[row] = sh.none ? 0.f : sh.bad ? NAN : loss;
+    P.lse[row] = sh.none ? 0.f : sum_lse(st, P.c, P.temperature);
+    if (P.stats) P.stats[row] = make_float2(st.m, sh.none ? 0.f : st.s);
+  }
+}
+
 template <int DT>
-__global__ void __launch_bounds__(kThreads) distill_forward_kernel(const __grid_constant__ RowsParams P) {
-  using T = typename El<DT>::T;
-  constexpr int V = El<DT>::kVec, U = 4;
-  __shared__ Stat red[kWarps];
-  __shared__ Stat mine;
-  __shared__ List list;
-  __shared__ int none;   // this row has no teacher: its logits need not be read
+__global__ void __launch_bounds__(kSumThreads + 32, kSumCtas) distill_forward_kernel(const __grid_constant__ RowsParams P) {
+  constexpr int S = kSumThreads;
+  __shared__ Shared<S> sh;
   const int parts = P.parts;
   const int64_t row = blockIdx.x / parts;
   const int part = (int)(blockIdx.x - row * parts);
   const int tid = threadIdx.x;
-  if (tid == 0) none = 0;
+  if (tid == 0) sh.none = 0;
   __syncthreads();
-
-  Teacher t;
-  if (tid >= kStream) {
-    t = read_list(list, P.list, row);
-    if (!t.any && (tid & 31) == 0) *(volatile int*)&none = 1;
-    if (part == 0) {
-      gather<DT>(list, static_cast<const T*>(P.z) + row * P.ld, P.list.top, 0, P.vocab);
-      list_softmax(list, P.list.top, P.c);
-    }
+  if (tid >= S) {
+    prepare_list<DT>(sh, P, row, 0, P.vocab);
   } else {
-    const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
-    Stat st{-INFINITY, 0.f};
-    const uint4* v = sp.vec();
-    int i = tid;
-    for (; i + (U - 1) * kStream < sp.n_vec; i += U * kStream) {
-      uint4 u[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) u[j] = __ldcs(v + i + j * kStream);
-      if (*(volatile int*)&none) break;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        float f[V];
-        El<DT>::unpack(u[j], f);
-        absorb(st, f, P.c);
-      }
-    }
-    for (; i < sp.n_vec; i += kStream) {
-      if (*(volatile int*)&none) break;
-      float f[V];
-      El<DT>::unpack(__ldcs(v + i), f);
-      absorb(st, f, P.c);
-    }
-    if (tid < sp.body - sp.lo) {
-      const float f[1] = {El<DT>::to(sp.row[sp.lo + tid])};
-      absorb(st, f, P.c);
-    }
-    if (tid < sp.hi - sp.tail()) {
-      const float f[1] = {El<DT>::to(sp.row[sp.tail() + tid])};
-      absorb(st, f, P.c);
-    }
-    block_stat(st, P.c, red);
+    const Stat st = warp_merge(sum_span<DT, S, kSumStep>(span_of<DT>(P, P.z, P.ld, row, part), P.c, &sh.none, false), P.c);
+    if ((tid & 31) == 0) sh.red[tid / 32] = st;
   }
-  __syncthreads();
-  Stat st;
-  if (parts > 1) {
-    if (tid == 0) mine = total_of(red, kWarps, P.c);
-    __syncwarp();
-    st = cluster_stat(&mine, parts, P.c);
-  } else if (tid >= kStream) {
-    st = total_of(red, kWarps, P.c);
-  }
-  if (tid >= kStream && part == 0) {
-    st = final_stat(st, t.bad);
-    const float loss = list_loss(list, P.list.top, st, P.c, P.temperature);
-    if ((tid & 31) == 0) {
-      if (!t.any) st.s = 0.f;
-      P.loss[row] = t.any ? (t.bad ? NAN : loss) : 0.f;
-      P.lse[row] = t.any ? st.m / P.temperature + logf(st.s) : 0.f;
-      if (P.stats) P.stats[row] = make_float2(st.m, st.s);
-    }
-  }
-  if (parts > 1) cluster_sync_all();   // no CTA leaves while its sum may still be read
+  finish_sum<S>(sh, parts, P.c);
+  if (tid >= S && part == 0) write_loss<S>(sh, P, row, final_stat(sh.total, sh.bad));
+  leave(parts);
 }
 
 // The gradient at the listed indices is A q - B (the sum of p over the entries with that
@@ -269,214 +336,166 @@ __device__ __forceinline__ void list_sums(List& s, int top) {
 template <int DT>
 __device__ __forceinline__ void patch(const List& s, int top, const Stat& st, float A, float B, float c,
                                       typename El<DT>::T* grad, int32_t lo, int32_t hi) {
+  const Base base(st.m, c);
   for (int k = threadIdx.x & 31; k < top; k += 32) {
     const int32_t i = s.idx[k];
-    if (i >= lo && i < hi) grad[i] = El<DT>::from(A * (ex2((s.z[k] - st.m) * c) / st.s) - B * s.lp[k]);
+    if (i >= lo && i < hi) grad[i] = El<DT>::from(A * (ex2(base.rel(s.z[k], c)) / st.s) - B * s.lp[k]);
   }
 }
 
-// dz = a 2^((z - m) c) over a span; the gradient's row has its own 16-byte phase.
-template <int DT> __device__ __forceinline__ float dense(float z, float m, float a, float c) { return a * ex2((z - m) * c); }
+// The dense part of a row's gradient, dz = a 2^((z - m) c) with a = A / s. For 16-bit gradients
+// |a| goes into the exponent, 2^(z c + k) with k = log2 |a| - mc, and the sign onto the rounded
+// pair: a multiplication less. Rounding k costs 2^-24 |k| of the result, so only where |mc| is at most
+// 64 (4e-6, a hundredth of fp16's half step).
+template <int DT> struct Dense {
+  static constexpr int V = El<DT>::kVec;
+  Base base;
+  float a, k;
+  uint32_t sign;
+  bool fold;
+
+  __device__ __forceinline__ Dense(const Stat& st, float A, float c) : base(st.m, c), a(A / st.s), k(0.f), sign(0), fold(false) {
+    if (DT != ZT_F32) {
+      if (a < 0.f) sign = 0x80008000u;
+      a = fabsf(a);
+      k = log2f(a) - base.mc;
+      fold = fabsf(base.mc) <= 64.f;
+    }
+  }
+  __device__ __forceinline__ typename El<DT>::T one(typename El<DT>::T z, float c) const {
+    const float v = fold ? ex2(__fmaf_rn(El<DT>::to(z), c, k)) : a * ex2(base.rel(El<DT>::to(z), c));
+    return El<DT>::from(sign ? -v : v);
+  }
+  __device__ __forceinline__ uint4 vec(const uint4& u, float c) const {
+    float f[V];
+    El<DT>::unpack(u, f);
+    if (DT != ZT_F32 && fold) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = ex2(__fmaf_rn(f[i], c, k));
+    } else if (!base.far()) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = a * ex2(__fmaf_rn(f[i], c, -base.mc));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = a * ex2((f[i] - base.m) * c);
+    }
+    uint4 r = El<DT>::pack(f);
+    if (DT != ZT_F32) {
+      r.x ^= sign; r.y ^= sign; r.z ^= sign; r.w ^= sign;
+    }
+    return r;
+  }
+};
+
+// The stream threads' part of a row's gradient over a span; `u` holds step 0, loaded before the
+// caller waited for anything, and each step is loaded before the one before it is written.
+// out has its own 16-byte phase.
+template <int DT, int S, int U>
+__device__ __forceinline__ void write_span(uint4 (&u)[U], const Span<DT>& sp, typename El<DT>::T* out, const Dense<DT>& D, float c) {
+  using T = typename El<DT>::T;
+  constexpr int V = El<DT>::kVec;
+  const int n = steps_of<DT, S, U>(sp), tid = threadIdx.x;
+  const bool same = ((uintptr_t)(out + sp.body) & 15) == 0;
+  uint4 next[U];
+  for (int g = 0; g < n; ++g) {
+    if (g + 1 < n) load_step<DT, S, U>(next, sp, g + 1, false);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = tid + (g * U + j) * S;
+      if (i < sp.n_vec) {
+        const uint4 r = D.vec(u[j], c);
+        if (same) {
+          __stcs(reinterpret_cast<uint4*>(out + sp.body) + i, r);
+        } else {   // an element at a time; in place this cannot be
+          const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+          for (int k = 0; k < V; ++k) out[sp.body + i * V + k] = e[k];
+        }
+      }
+      u[j] = next[j];
+    }
+  }
+  if (tid < sp.body - sp.lo) out[sp.lo + tid] = D.one(sp.row[sp.lo + tid], c);
+  if (tid < sp.hi - sp.tail()) out[sp.tail() + tid] = D.one(sp.row[sp.tail() + tid], c);
+}
+
+template <int DT, int S>
+__device__ __forceinline__ void zero_span(const Span<DT>& sp, typename El<DT>::T* out) {
+  for (int i = sp.lo + threadIdx.x; i < sp.hi; i += S) out[i] = El<DT>::from(0.f);
+}
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) distill_backward_kernel(const __grid_constant__ RowsParams P) {
+__global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backward_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
-  constexpr int V = El<DT>::kVec, U = 4;
+  constexpr int S = kWriteThreads, U = kWriteStep;
+  __shared__ List list;
   // last rows first: those the forward read last may still be in L2
   const unsigned place = gridDim.x - 1 - blockIdx.x;
   const int64_t row = place / P.parts;
   const int part = (int)(place - row * P.parts);
   const int tid = threadIdx.x;
+  const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
+  uint4 u[U];
+  if (tid < S) load_step<DT, S, U>(u, sp, 0, false);
   const float2 s2 = P.stats[row];
   const Stat st{s2.x, s2.y};
-  const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
   T* out = static_cast<T*>(P.grad) + row * P.ld_grad;
   const bool none = st.s == 0.f;
-  const float g = P.g ? P.g[row] : 0.f, gl = P.g_lse ? P.g_lse[row] : 0.f;
-  const float B = g * P.temperature, A = B + gl / P.temperature;
-  const bool in_place = P.grad == P.z;
-
-  __shared__ List list;
-  if (tid >= kStream && !none) {
+  const float B = (P.g ? P.g[row] : 0.f) * P.temperature, A = B + (P.g_lse ? P.g_lse[row] / P.temperature : 0.f);
+  if (tid >= S && !none) {
     read_list(list, P.list, row);
     gather<DT>(list, sp.row, P.list.top, sp.lo, sp.hi);
     list_softmax(list, P.list.top, P.c);
     list_sums(list, P.list.top);
   }
-  if (in_place) __syncthreads();   // the listed logits are read before they are overwritten
-  if (tid < kStream) {
-    const float a = A / st.s;
-    const uint4* v = sp.vec();
-    const bool same = ((uintptr_t)(out + sp.body) & 15) == 0;
-    if (none) {
-      for (int i = sp.lo + tid; i < sp.hi; i += kStream) out[i] = El<DT>::from(0.f);
-    } else if (same) {
-      uint4* o = reinterpret_cast<uint4*>(out + sp.body);
-      int i = tid;
-      for (; i + (U - 1) * kStream < sp.n_vec; i += U * kStream) {
-        uint4 u[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) u[j] = __ldcs(v + i + j * kStream);
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          float f[V];
-          El<DT>::unpack(u[j], f);
-#pragma unroll
-          for (int k = 0; k < V; ++k) f[k] = dense<DT>(f[k], st.m, a, P.c);
-          __stcs(o + i + j * kStream, El<DT>::pack(f));
-        }
-      }
-      for (; i < sp.n_vec; i += kStream) {
-        float f[V];
-        El<DT>::unpack(__ldcs(v + i), f);
-#pragma unroll
-        for (int k = 0; k < V; ++k) f[k] = dense<DT>(f[k], st.m, a, P.c);
-        __stcs(o + i, El<DT>::pack(f));
-      }
-      if (tid < sp.body - sp.lo) out[sp.lo + tid] = El<DT>::from(dense<DT>(El<DT>::to(sp.row[sp.lo + tid]), st.m, a, P.c));
-      if (tid < sp.hi - sp.tail())
-        out[sp.tail() + tid] = El<DT>::from(dense<DT>(El<DT>::to(sp.row[sp.tail() + tid]), st.m, a, P.c));
-    } else {
-      for (int i = sp.lo + tid; i < sp.hi; i += kStream) out[i] = El<DT>::from(dense<DT>(El<DT>::to(sp.row[i]), st.m, a, P.c));
-    }
+  if (P.grad == P.z) __syncthreads();   // in place: the listed logits are read before they are overwritten
+  if (tid < S) {
+    if (none) zero_span<DT, S>(sp, out);
+    else write_span<DT, S, U>(u, sp, out, Dense<DT>(st, A, P.c), P.c);
   }
   __syncthreads();
-  if (tid >= kStream && !none) patch<DT>(list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
+  if (tid >= S && !none) patch<DT>(list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
 }
 
-// Loss and gradient at once: a cluster's CTAs hold the row, so it is read once. A thread
-// copies its own vectors to shared memory (cp.async: no registers, no barrier), adds them up
-// as they land, and after the cluster has merged its sums turns the same vectors into the
-// gradient.
-__device__ __forceinline__ void copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(zt::tc::smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
+// Loss and gradient at once: the sum reads the row from memory, the gradient reads it again from
+// L2. (Held in the shared memory of a cluster of four instead, the row's loads, sums and
+// stores took turns, and 2048 x 128256 bf16 measured 256 us against 227.)
 template <int DT>
-__global__ void __launch_bounds__(kThreads) distill_grad_kernel(const __grid_constant__ RowsParams P) {
+__global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_grad_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
-  constexpr int V = El<DT>::kVec, U = 2, D = 8;   // D groups of U vectors a thread in flight
-  extern __shared__ uint4 held[];
-  __shared__ Stat red[kWarps];
-  __shared__ Stat mine;
-  __shared__ List list;
-  __shared__ int none, bad;   // no teacher; an index that does not exist
+  constexpr int S = kWriteThreads, U = kWriteStep;
+  __shared__ Shared<S> sh;
   const int parts = P.parts;
   const int64_t row = blockIdx.x / parts;
   const int part = (int)(blockIdx.x - row * parts);
   const int tid = threadIdx.x;
   const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
-  const uint4* v = sp.vec();
-  if (tid < kStream) {   // the first groups are on their way before anything else
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = tid + (d * U + j) * kStream;
-        if (i < sp.n_vec) copy16(held + i, v + i);
-      }
-      copy_commit();
-    }
-  }
-  if (tid == 0) none = 0;
+  if (tid == 0) sh.none = 0;
   __syncthreads();
-
-  float head = 0.f, tail = 0.f;   // the elements before and behind the vectors
-  if (tid >= kStream) {
-    const Teacher t = read_list(list, P.list, row);
-    if ((tid & 31) == 0) {
-      bad = t.bad;
-      if (!t.any) *(volatile int*)&none = 1;
-    }
-    gather<DT>(list, static_cast<const T*>(P.z) + row * P.ld, P.list.top, 0, P.vocab);
-    list_softmax(list, P.list.top, P.c);
+  uint4 u[U];
+  if (tid >= S) {
+    prepare_list<DT>(sh, P, row, 0, P.vocab);   // in place: all of it before any part writes
   } else {
-    Stat st{-INFINITY, 0.f};
-    if (tid < sp.body - sp.lo) {
-      head = El<DT>::to(sp.row[sp.lo + tid]);
-      const float f[1] = {head};
-      absorb(st, f, P.c);
-    }
-    if (tid < sp.hi - sp.tail()) {
-      tail = El<DT>::to(sp.row[sp.tail() + tid]);
-      const float f[1] = {tail};
-      absorb(st, f, P.c);
-    }
-    for (int g = 0; g * U * kStream < sp.n_vec; ++g) {
-      copy_wait<D - 1>();
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = tid + (g * U + j) * kStream;
-        if (i < sp.n_vec) {
-          float f[V];
-          El<DT>::unpack(held[i], f);
-          absorb(st, f, P.c);
-        }
-      }
-      if (!*(volatile int*)&none) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          const int i = tid + ((g + D) * U + j) * kStream;
-          if (i < sp.n_vec) copy16(held + i, v + i);
-        }
-      }
-      copy_commit();
-    }
-    copy_wait<0>();
-    block_stat(st, P.c, red);
+    const Stat st = warp_merge(sum_span<DT, S, U>(sp, P.c, &sh.none, true), P.c);
+    if ((tid & 31) == 0) sh.red[tid / 32] = st;
+    load_step<DT, S, U>(u, sp, 0, false);
   }
-  __syncthreads();
-  Stat st;
-  if (parts > 1) {
-    if (tid == 0) mine = total_of(red, kWarps, P.c);
-    __syncwarp();
-    st = cluster_stat(&mine, parts, P.c);
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this thread has read the peers' sums
-  } else {
-    st = total_of(red, kWarps, P.c);
-  }
+  finish_sum<S>(sh, parts, P.c);
+  const bool none = sh.none;
+  const Stat st = final_stat(sh.total, sh.bad);
   const float B = P.g[row] * P.temperature, A = B + (P.g_lse ? P.g_lse[row] / P.temperature : 0.f);
   T* out = static_cast<T*>(P.grad) + row * P.ld_grad;
-  const bool any = !none;
-  st = final_stat(st, bad);
-  if (tid >= kStream) {
-    if (part == 0) {
-      const float loss = list_loss(list, P.list.top, st, P.c, P.temperature);
-      if ((tid & 31) == 0) {
-        P.loss[row] = any ? (bad ? NAN : loss) : 0.f;
-        P.lse[row] = any ? st.m / P.temperature + logf(st.s) : 0.f;
-      }
-    }
-    list_sums(list, P.list.top);   // after the loss: it takes the place of log2 p
+  if (tid >= S) {
+    if (part == 0) write_loss<S>(sh, P, row, st);
+    list_sums(sh.list, P.list.top);   // after the loss: it takes the place of log2 p
+  } else if (none) {
+    zero_span<DT, S>(sp, out);
   } else {
-    const float a = A / st.s;
-    const bool same = ((uintptr_t)(out + sp.body) & 15) == 0;
-    if (!any) {
-      for (int i = sp.lo + tid; i < sp.hi; i += kStream) out[i] = El<DT>::from(0.f);
-    } else {
-      uint4* o = reinterpret_cast<uint4*>(out + sp.body);
-      for (int i = tid; i < sp.n_vec; i += kStream) {
-        float f[V];
-        El<DT>::unpack(held[i], f);
-#pragma unroll
-        for (int k = 0; k < V; ++k) f[k] = dense<DT>(f[k], st.m, a, P.c);
-        if (same) {
-          __stcs(o + i, El<DT>::pack(f));
-        } else {
-          T* e = out + sp.body + i * V;
-#pragma unroll
-          for (int k = 0; k < V; ++k) e[k] = El<DT>::from(f[k]);
-        }
-      }
-      if (tid < sp.body - sp.lo) out[sp.lo + tid] = El<DT>::from(dense<DT>(head, st.m, a, P.c));
-      if (tid < sp.hi - sp.tail()) out[sp.tail() + tid] = El<DT>::from(dense<DT>(tail, st.m, a, P.c));
-    }
+    write_span<DT, S, U>(u, sp, out, Dense<DT>(st, A, P.c), P.c);
   }
   __syncthreads();
-  if (tid >= kStream && any) patch<DT>(list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
-  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // no CTA leaves while its sum may be read
+  if (tid >= S && !none) patch<DT>(sh.list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
+  leave(parts);
 }
 
 int check_rows(const zt_distill_args* a, bool grad, const std::string& who) {
@@ -498,14 +517,29 @@ int check_rows(const zt_distill_args* a, bool grad, const std::string& who) {
   return ZT_OK;
 }
 
-// CTAs of a row: 1 where the rows alone fill the SMs twice, else the power of two up to 8
-// that does, while a part still has kMinPart elements (below that a part is all latency).
-constexpr int kMinPart = 2048;
+// CTAs of a row: doubled up to 8 while all of them still run at once, and a part keeps at least
+// kMinPart elements. (Splitting rows that fill the GPU's slots already, to even out their last
+// wave, costs more than it gives: 1001 x 50257 fp16 forward 34 us in two parts, 28 in one.)
+constexpr int64_t kMinPart = 2048;
 
-int parts_for(int64_t rows, int64_t vocab) {
-  const int64_t want = 2 * (int64_t)zt::sm_count();
+int parts_for(const zt_distill_args* a, int ctas) {
+  const int64_t slots = (int64_t)zt::sm_count() * ctas;
   int parts = 1;
-  while (parts < kMaxCluster && rows * parts < want && vocab / (2 * parts) >= kMinPart) parts *= 2;
+  while (parts < kMaxCluster && 2 * parts * a->rows <= slots && a->vocab / (2 * parts) >= kMinPart) parts *= 2;
+  return parts;
+}
+
+int64_t row_bytes(const zt_distill_args* a) { return a->vocab * (a->dtype == ZT_F32 ? 4 : 2); }
+
+// The same for loss and gradient at once, whose rows under way have to stay in L2 between their
+// two readings: at most kInFlight bytes of them (of 2048 x 128256 bf16, 76 MB under way
+// measured 227 us, 151 MB 254).
+constexpr int64_t kInFlight = 80ll << 20;
+
+int parts_for_grad(const zt_distill_args* a) {
+  const int64_t slots = (int64_t)zt::sm_count() * kWriteCtas;
+  int parts = parts_for(a, kWriteCtas);
+  while (parts < kMaxCluster && slots / parts * row_bytes(a) > kInFlight && a->rows * parts >= slots) parts *= 2;
   return parts;
 }
 
@@ -529,11 +563,11 @@ RowsParams rows_params(const zt_distill_args* a, int parts) {
   return P;
 }
 
-template <class K> int launch(K kernel, const RowsParams& P, int64_t rows, bool cluster, size_t smem, cudaStream_t s, const char* who) {
+template <class K>
+int launch(K kernel, int threads, const RowsParams& P, int64_t rows, bool cluster, cudaStream_t s, const char* who) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * P.parts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
   if (cluster && P.parts > 1) {
@@ -546,49 +580,6 @@ template <class K> int launch(K kernel, const RowsParams& P, int64_t rows, bool 
   return zt::check_cuda(cudaLaunchKernelEx(&cfg, kernel, P), who);
 }
 
-int forward(const zt_distill_args* a, cudaStream_t s, const char* who) {
-  const RowsParams P = rows_params(a, parts_for(a->rows, a->vocab));
-  if (a->dtype == ZT_BF16) return launch(distill_forward_kernel<ZT_BF16>, P, a->rows, true, 0, s, who);
-  if (a->dtype == ZT_F16) return launch(distill_forward_kernel<ZT_F16>, P, a->rows, true, 0, s, who);
-  return launch(distill_forward_kernel<ZT_F32>, P, a->rows, true, 0, s, who);
-}
-
-int backward(const zt_distill_args* a, cudaStream_t s, const char* who) {
-  const RowsParams P = rows_params(a, parts_for(a->rows, a->vocab));
-  if (a->dtype == ZT_BF16) return launch(distill_backward_kernel<ZT_BF16>, P, a->rows, false, 0, s, who);
-  if (a->dtype == ZT_F16) return launch(distill_backward_kernel<ZT_F16>, P, a->rows, false, 0, s, who);
-  return launch(distill_backward_kernel<ZT_F32>, P, a->rows, false, 0, s, who);
-}
-
-// A part of distill_grad_kernel's row in shared memory: 64 KB leave room for three CTAs on an
-// SM, whose loads, sums and stores overlap; longer rows take up to kMaxPart in each of
-// eight parts, and rows beyond that the forward and the backward kernel.
-constexpr size_t kGoodPart = 64 * 1024;
-constexpr size_t kMaxPart = 200 * 1024;
-
-size_t part_bytes(const zt_distill_args* a, int parts) {
-  const size_t len = (size_t)(((a->vocab + parts - 1) / parts + 7) / 8 * 8);
-  return len * (a->dtype == ZT_F32 ? 4 : 2);
-}
-
-template <int DT> int grad_once(const RowsParams& P, int64_t rows, size_t smem, cudaStream_t s) {
-  static std::mutex mu;
-  static bool ready[64] = {false};
-  int dev = 0;
-  if (int rc = zt::check_cuda(cudaGetDevice(&dev), "zt_distill_rows_grad: cudaGetDevice")) return rc;
-  if (dev < 0 || dev >= 64) return zt::set_error(ZT_ERR_LIMIT, "zt_distill_rows_grad: device ordinal >= 64");
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!ready[dev]) {
-      if (int rc = zt::check_cuda(cudaFuncSetAttribute(distill_grad_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       (int)kMaxPart), "zt_distill_rows_grad: shared memory attribute"))
-        return rc;
-      ready[dev] = true;
-    }
-  }
-  return launch(distill_grad_kernel<DT>, P, rows, true, smem, s, "zt_distill_rows_grad launch");
-}
-
 }  // namespace
 
 extern "C" {
@@ -598,7 +589,10 @@ int zt_distill_rows(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, false, "zt_distill_rows")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->loss || !a->lse) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows: null pointer");
-  return forward(a, zt::as_stream(stream), "zt_distill_rows launch");
+  const RowsParams P = rows_params(a, parts_for(a, kSumCtas));
+  auto* kernel = a->dtype == ZT_BF16 ? distill_forward_kernel<ZT_BF16>
+                 : a->dtype == ZT_F16 ? distill_forward_kernel<ZT_F16> : distill_forward_kernel<ZT_F32>;
+  return launch(kernel, kSumThreads + 32, P, a->rows, true, zt::as_stream(stream), "zt_distill_rows launch");
 }
 
 int zt_distill_rows_backward(const zt_distill_args* a, void* stream) {
@@ -606,26 +600,21 @@ int zt_distill_rows_backward(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, true, "zt_distill_rows_backward")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->stats) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_backward: null pointer");
-  return backward(a, zt::as_stream(stream), "zt_distill_rows_backward launch");
+  const RowsParams P = rows_params(a, parts_for(a, kWriteCtas));
+  auto* kernel = a->dtype == ZT_BF16 ? distill_backward_kernel<ZT_BF16>
+                 : a->dtype == ZT_F16 ? distill_backward_kernel<ZT_F16> : distill_backward_kernel<ZT_F32>;
+  return launch(kernel, kWriteThreads + 32, P, a->rows, false, zt::as_stream(stream), "zt_distill_rows_backward launch");
 }
 
 int zt_distill_rows_grad(const zt_distill_args* a, void* stream) {
   zt::clear_error();
   if (int rc = check_rows(a, true, "zt_distill_rows_grad")) return rc;
   if (a->rows == 0) return ZT_OK;
-  if (!a->loss || !a->lse || !a->stats || !a->weight) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_grad: null pointer");
-  int parts = parts_for(a->rows, a->vocab);
-  while (parts < kMaxCluster && part_bytes(a, parts) > kGoodPart) parts *= 2;
-  const size_t smem = part_bytes(a, parts);
-  cudaStream_t s = zt::as_stream(stream);
-  if (smem > kMaxPart) {   // the row does not fit a cluster's shared memory
-    if (int rc = forward(a, s, "zt_distill_rows_grad launch")) return rc;
-    return backward(a, s, "zt_distill_rows_grad launch");
-  }
-  const RowsParams P = rows_params(a, parts);
-  if (a->dtype == ZT_BF16) return grad_once<ZT_BF16>(P, a->rows, smem, s);
-  if (a->dtype == ZT_F16) return grad_once<ZT_F16>(P, a->rows, smem, s);
-  return grad_once<ZT_F32>(P, a->rows, smem, s);
+  if (!a->loss || !a->lse || !a->weight) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_grad: null pointer");
+  const RowsParams P = rows_params(a, parts_for_grad(a));
+  auto* kernel = a->dtype == ZT_BF16 ? distill_grad_kernel<ZT_BF16>
+                 : a->dtype == ZT_F16 ? distill_grad_kernel<ZT_F16> : distill_grad_kernel<ZT_F32>;
+  return launch(kernel, kWriteThreads + 32, P, a->rows, true, zt::as_stream(stream), "zt_distill_rows_grad launch");
 }
 
 }  // extern "C"

@@ -18,12 +18,40 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// sum over v of 2^((z_v - m) c) as (m, s). The maximum is subtracted before the scaling, so
-// that a logit at its type's lowest value gives 2^-inf = 0 and a row of nothing but such
-// values stays finite.
+// A sum over v of 2^((z_v - m) c) as (m, s). m is a z near the largest one: it follows the
+// running maximum only when that is more than kSlack powers of two ahead, because with a running
+// maximum of their own some lane of a warp has a new one at almost every step, and the rescaling
+// measured a third of the instructions. A sum of 2^30 such terms stays below 2^47.
+//
+// (z - m) c is fma(z, c, -mc) with mc = round(m c): one instruction, and its rounding of m c is
+// the same for every term, so that it cancels as long as all uses of a sum take the same mc
+// (merging two sums multiplies by 2^(mc - mc'), and logs of q are relative to mc). Beyond
+// kFar, where z c may leave the range (a logit at its type's lowest value), the
+// difference is taken first: such a logit gives 2^-inf = 0, and a row of nothing else stays
+// finite.
 struct Stat {
   float m, s;
 };
+
+constexpr float kFar = 1e30f;
+constexpr float kSlack = 16.f;
+
+struct Base {
+  float m, mc;   // 0 where there is no finite maximum yet
+  __device__ __forceinline__ Base(float max, float c) {
+    m = max == -INFINITY ? 0.f : max;
+    mc = __fmul_rn(m, c);
+  }
+  __device__ __forceinline__ bool far() const { return fabsf(m) > kFar; }
+  __device__ __forceinline__ float rel(float z, float c) const { return far() ? (z - m) * c : __fmaf_rn(z, c, -mc); }
+};
+
+// The factor that takes a sum from base a to the larger b.
+__device__ __forceinline__ float rescale(float a, float b, float c) {
+  if (a == -INFINITY) return 0.f;
+  if (fabsf(a) > kFar || fabsf(b) > kFar) return ex2((a - b) * c);
+  return ex2(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, c)));
+}
 
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float c) {
   Stat r;
@@ -31,7 +59,7 @@ __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float c) {
   if (r.m == -INFINITY) {
     r.s = a.s + b.s;   // nothing on either side, or NaN
   } else {
-    r.s = a.s * ex2((a.m - r.m) * c) + b.s * ex2((b.m - r.m) * c);
+    r.s = a.s * rescale(a.m, r.m, c) + b.s * rescale(b.m, r.m, c);
   }
   return r;
 }
@@ -47,23 +75,29 @@ __device__ __forceinline__ Stat warp_merge(Stat v, float c) {
   return v;
 }
 
-// N values into a running (m, s).
+// N values, cm the largest of them, into a running (m, s).
+template <int N> __device__ __forceinline__ void absorb(Stat& st, const float (&f)[N], float cm, float c) {
+  if (cm > st.m + kSlack / c) {   // and wherever m is still -inf
+    st.s *= rescale(st.m, cm, c);
+    st.m = cm;
+  }
+  const Base base(st.m, c);
+  float a[2] = {0.f, 0.f};
+  if (base.far()) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i & 1] += ex2((f[i] - base.m) * c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i & 1] += ex2(__fmaf_rn(f[i], c, -base.mc));
+  }
+  st.s += a[0] + a[1];
+}
+
 template <int N> __device__ __forceinline__ void absorb(Stat& st, const float (&f)[N], float c) {
   float cm = f[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) cm = fmaxf(cm, f[i]);
-  if (cm > st.m) {
-    st.s *= ex2((st.m - cm) * c);
-    st.m = cm;
-  }
-  const float base = st.m == -INFINITY ? 0.f : st.m;
-  float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    a0 += ex2((f[i] - base) * c);
-    if (i + 1 < N) a1 += ex2((f[i + 1] - base) * c);
-  }
-  st.s += a0 + a1;
+  absorb(st, f, cm, c);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -89,7 +123,7 @@ struct TopList {
 // A row's list in shared memory, worked on by one warp: lane l owns entries l, l + 32, ...
 // An entry with a negative index or the value -inf carries no mass and its other half is not
 // looked at.
-struct List {
+struct alignas(16) List {
   int32_t idx[kMaxTop];   // -1: no mass
   float p[kMaxTop];       // teacher probability, 0 without mass
   float lp[kMaxTop];      // its log2, 0 where p is 0
@@ -167,12 +201,19 @@ __device__ __forceinline__ void list_softmax(List& s, int top, float c) {
   }
 }
 
+// log sum_v exp(z_v / T) of a finished sum.
+__device__ __forceinline__ float sum_lse(const Stat& st, float c, float temperature) {
+  const Base base(st.m, c);
+  return base.far() ? st.m / temperature + logf(st.s) : fmaf(base.mc, kLn2, logf(st.s));
+}
+
 // T^2 sum_k p_k (log p_k - log q_k) from the list and the logits at its indices.
 __device__ __forceinline__ float list_loss(const List& s, int top, const Stat& st, float c, float temperature) {
   const float ls = log2f(st.s);
+  const Base base(st.m, c);
   float a = 0.f;
   for (int k = threadIdx.x & 31; k < top; k += 32)
-    if (s.p[k] != 0.f) a = fmaf(s.p[k], s.lp[k] - ((s.z[k] - st.m) * c - ls), a);
+    if (s.p[k] != 0.f) a = fmaf(s.p[k], s.lp[k] - (base.rel(s.z[k], c) - ls), a);
   return warp_sum(a) * (kLn2 * temperature * temperature);
 }
 

@@ -71,13 +71,18 @@ __global__ void __launch_bounds__(32 * kListWarps) list_kernel(const __grid_cons
   list_softmax(s, P.top, P.c);
   for (int k = lane; k < P.top; k += 32)
     if (s.p[k] == 0.f) s.idx[k] = INT32_MAX;   // no mass: behind the others
+  if (lane < (-P.top & 3)) s.idx[P.top + lane] = INT32_MAX;   // up to a whole 16 bytes
   __syncwarp();
   // an entry's place: those with a smaller token, or the same and an earlier place
   for (int k = lane; k < P.top; k += 32) {
     const int32_t own = s.idx[k];
     int place = 0;
-#pragma unroll 8
-    for (int j = 0; j < P.top; ++j) place += (s.idx[j] < own || (s.idx[j] == own && j < k)) ? 1 : 0;
+#pragma unroll 4
+    for (int j = 0; j < P.top; j += 4) {   // behind the list stands INT32_MAX: never before an entry
+      const int4 o = *reinterpret_cast<const int4*>(s.idx + j);
+      place += (o.x < own || (o.x == own && j < k)) + (o.y < own || (o.y == own && j + 1 < k)) +
+               (o.z < own || (o.z == own && j + 2 < k)) + (o.w < own || (o.w == own && j + 3 < k));
+    }
     const int64_t at = row * P.top + place;
     P.idx[at] = own;
     P.lp[at] = s.lp[k];
@@ -245,9 +250,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + b * kTile;
         const int tile0 = nt * kTile;
         for (;;) {  // the listed columns of this tile, one column of the warp's rows at a time
-          const unsigned has = __ballot_sync(0xffffffffu, next < tile0 + kTile);
-          if (!has) break;
-          const int col = __shfl_sync(0xffffffffu, next, __ffs(has) - 1);
+          const int col = __reduce_min_sync(0xffffffffu, next);   // each column once, in order
+          if (col >= tile0 + kTile) break;
           const float v = tmem_ld1(acc + (uint32_t)(col - tile0));
           if (next == col) {
             P.z[(int64_t)row * P.top + pos] = v;
@@ -287,39 +291,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// 32 rows a block. Warp w merges splits w, w + kListWarps, ... of the rows, lane = row, so that
-// a warp reads 256 adjacent bytes; then each warp takes the lists of four rows.
+// Eight rows a block. Its threads merge the rows' splits (eight adjacent rows, 64 bytes, a group
+// of eight threads), then a warp takes a row's list, which it loaded before.
+constexpr int kCombineRows = kListWarps;
+
 __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_constant__ Params P) {
-  __shared__ Stat part[kListWarps][32];
-  const int64_t row0 = (int64_t)blockIdx.x * 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  __shared__ Stat part[kListWarps][kCombineRows];
+  const int64_t row0 = (int64_t)blockIdx.x * kCombineRows;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+  const int64_t row = row0 + warp;
+  constexpr int kHeld = 4;   // list entries of a lane loaded ahead
+  int32_t idx[kHeld], status = kNoTeacher;
+  float lp[kHeld], z[kHeld];
+#pragma unroll
+  for (int e = 0; e < kHeld; ++e) {
+    idx[e] = INT32_MAX;
+    if (row < P.rows && lane + 32 * e < P.top) {
+      const int64_t at = row * P.top + lane + 32 * e;
+      idx[e] = __ldg(P.idx + at);
+      lp[e] = __ldg(P.lp + at);
+      z[e] = __ldg(P.z + at);   // not written where idx is INT32_MAX, and then not looked at
+    }
+  }
+  if (row < P.rows) status = __ldg(P.status + row);
   Stat st{-INFINITY, 0.f};
 #pragma unroll 4
-  for (int sp = warp; sp < P.n_splits; sp += kListWarps) {   // rows_pad covers row0 + lane
-    const float2 o = P.partials[(size_t)sp * P.rows_pad + row0 + lane];
+  for (int sp = tid / kCombineRows; sp < P.n_splits; sp += 32 * kListWarps / kCombineRows) {   // rows_pad covers the block
+    const float2 o = __ldg(P.partials + (size_t)sp * P.rows_pad + row0 + tid % kCombineRows);
     st = merge(st, Stat{o.x, o.y}, P.c);
   }
-  part[warp][lane] = st;
-  __syncthreads();
-  for (int r = warp; r < 32; r += kListWarps) {
-    const int64_t row = row0 + r;
-    if (row >= P.rows) break;
-    st = part[0][r];
 #pragma unroll
-    for (int w = 1; w < kListWarps; ++w) st = merge(st, part[w][r], P.c);
-    if (st.m == -INFINITY) st.s = NAN;
-    const float ls = log2f(st.s);
-    float a = 0.f;
-    for (int k = lane; k < P.top; k += 32) {
-      const int64_t at = row * P.top + k;
-      if (P.idx[at] != INT32_MAX) a = fmaf(exp2f(P.lp[at]), P.lp[at] - ((P.z[at] - st.m) * P.c - ls), a);
-    }
-    a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
-    if (lane == 0) {
-      const int32_t status = P.status[row];
-      P.loss[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : a;
-      P.lse[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : st.m / P.temperature + logf(st.s);
-    }
+  for (int o = kCombineRows; o < 32; o <<= 1) {
+    Stat u;
+    u.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    u.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    st = merge(st, u, P.c);
+  }
+  if (lane < kCombineRows) part[warp][lane] = st;
+  __syncthreads();
+  if (row >= P.rows) return;
+  st = part[0][warp];
+#pragma unroll
+  for (int w = 1; w < kListWarps; ++w) st = merge(st, part[w][warp], P.c);
+  if (st.m == -INFINITY) st.s = NAN;
+  const float ls = log2f(st.s);
+  const Base base(st.m, P.c);
+  float a = 0.f;
+  auto add = [&](float l, float v) { a = fmaf(exp2f(l), l - (base.rel(v, P.c) - ls), a); };
+#pragma unroll
+  for (int e = 0; e < kHeld; ++e)
+    if (idx[e] != INT32_MAX) add(lp[e], z[e]);
+  for (int k = lane + 32 * kHeld; k < P.top; k += 32) {
+    const int64_t at = row * P.top + k;
+    if (P.idx[at] != INT32_MAX) add(P.lp[at], P.z[at]);
+  }
+  a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
+  if (lane == 0) {
+    P.loss[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : a;
+    P.lse[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : sum_lse(st, P.c, P.temperature);
   }
 }
 
@@ -476,7 +505,7 @@ int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
   if (int rc = zt::check_cuda(cudaGetLastError(), "zt_linear_distill: list launch")) return rc;
   linear_distill_kernel<<<2 * clusters, kThreads, kSmem, s>>>(P);
   if (int rc = zt::check_cuda(cudaGetLastError(), "zt_linear_distill: gemm launch")) return rc;
-  combine_kernel<<<(unsigned)((a->rows + 31) / 32), 32 * kListWarps, 0, s>>>(P);
+  combine_kernel<<<(unsigned)((a->rows + kCombineRows - 1) / kCombineRows), 32 * kListWarps, 0, s>>>(P);
   return zt::check_cuda(cudaGetLastError(), "zt_linear_distill: combine launch");
 }
 

@@ -1251,10 +1251,10 @@ def distill_rows_grad(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: t
             raise ValueError("out overlaps the teacher's lists or the weights")
         if not out.is_inference():
             torch.autograd.graph.increment_version(out)
-    buf = x.new_empty((4, rows), dtype=torch.float32)   # loss, lse and what a row's two passes share
+    buf = x.new_empty((2, rows), dtype=torch.float32)
     at = buf.data_ptr()
     _distill_call("zt_distill_rows_grad", x, top_idx, top_logits, temperature, grad=out, weight=weight.contiguous(), loss=at,
-                  lse=at + 4 * rows, stats=at + 8 * rows)
+                  lse=at + 4 * rows)
     return buf[0], buf[1], out
 
 
