@@ -376,7 +376,9 @@ int prepare(int dev) {
 }
 
 // Vocabulary split: the split length (in 256-column tiles) whose round-robin schedule over
-// `pairs` CTA pairs has the smallest longest queue, preferring longer splits on ties.
+// `pairs` CTA pairs has the shortest longest queue, an item counting an eighth of a tile more than
+// its tiles: at its start every row looks up its place in its list, and at its end leaves
+// a partial sum to be merged (8192 x 128256 rows in splits of one tile: 33 MB of them).
 struct Split {
   int32_t m_tiles, n_tiles, split_tiles, n_splits, rows_pad;
 };
@@ -391,7 +393,7 @@ Split choose_split(int64_t rows, int64_t vocab, int pairs) {
   for (int st = 1; st <= sp.n_tiles && st <= 64; ++st) {
     const long long splits = (sp.n_tiles + st - 1) / st;
     const long long items = splits * sp.m_tiles;
-    const long long queue = (items + pairs - 1) / pairs * st;
+    const long long queue = (items + pairs - 1) / pairs * (8 * st + 1);
     if (best < 0 || queue <= best) {
       best = queue;
       sp.split_tiles = st;

@@ -28,9 +28,9 @@ namespace {
 constexpr int kWarps = 4;          // warps of a forward block; they share nothing
 constexpr int kBwdWarps = 8;       // warps of a backward block; they share the weight gradient's sum
 constexpr int kBwdBlocks = 2;      // of them on an SM
-constexpr int kFwdBlocks = 5;      // ring kernels: forward blocks on an SM, and the steps a warp has in flight
+constexpr int kFwdBlocks = 3;      // ring kernels: forward blocks on an SM, and the steps a warp has in flight
 constexpr int kFwdRing = 8;
-constexpr int kBwdRing = 4;
+constexpr int kBwdRing = 2;
 constexpr int kMaxHeadDim = 512;   // 32 lanes x 8 elements of each half
 constexpr int kE = 8;              // elements of each half that a lane holds at most
 
@@ -458,11 +458,51 @@ template <class T, bool GRAD> struct Cursor {
   }
 };
 
+// cos and sin of a position, a lane's pieces: of the heads' type they are loaded a position ahead
+// and kept packed until they are used; fp32 ones of 16-bit heads are loaded where they are used.
+template <int DT> struct Tables {
+  static constexpr int V = DT == ZT_F32 ? 4 : 8;
+  Piece<DT, V, 1> piece[4];   // cos, cos', sin, sin'
+  int64_t row;
+
+  __device__ __forceinline__ void fetch(const QkParams& P, const Item& it, int sub, int lanes) {
+    using T = typename El<DT>::T;
+    row = (int64_t)(P.per_batch ? it.row : it.t) * P.hd;
+    if (P.t_dtype == DT) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        piece[i].load(static_cast<const T*>(i < 2 ? P.cos : P.sin) + row + (i & 1) * P.half, sub, lanes, P.half);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[V], int i, const QkParams& P, int sub, int lanes) const {
+    if (P.t_dtype == DT) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = piece[i].at(0, j);
+    } else {
+      load_side<DT, V, 1>(reinterpret_cast<float(&)[1][V]>(v), i < 2 ? P.cos : P.sin, row + (i & 1) * P.half, P.t_dtype, sub,
+                          lanes, P.half);
+    }
+  }
+};
+
+// The block's copy of both norm weights, widened: lane-wise as the heads are.
+template <int DT> struct Weights {
+  static constexpr int kV = DT == ZT_F32 ? 4 : 8;
+  float w[2][2][kV / 4][32][4];   // of q and k, both halves
+
+  __device__ __forceinline__ void fill(const QkParams& P, int warp, int lane, int sub, int lanes) {   // the first four warps
+    float v[1][kV];
+    load_side<DT, kV, 1>(v, P.w[warp / 2], (warp & 1) * P.half, P.w_dtype, sub, lanes, P.half);
+    smem_put(smem_at(&w[warp / 2][warp & 1][0][lane]), v[0]);
+  }
+};
+
 template <int DT, int LANES>
 __global__ void __launch_bounds__(32 * kWarps, kFwdBlocks) qk_forward_ring_kernel(const __grid_constant__ QkParams P) {
   using T = typename El<DT>::T;
   constexpr int V = 16 / (int)sizeof(T), D = kFwdRing;
   __shared__ uint4 rings[kWarps][D][2][32];
+  __shared__ Weights<DT> weights;
   const int lanes = LANES > 0 ? LANES : P.lanes, per_warp = 32 / lanes;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, sub = lane & (lanes - 1), mine = lane / lanes;
   const uint32_t ring = smem_at(&rings[warp][0][0][lane]);   // a step's slot is 1024 bytes
@@ -484,32 +524,38 @@ __global__ void __launch_bounds__(32 * kWarps, kFwdBlocks) qk_forward_ring_kerne
   };
 #pragma unroll 1
   for (int d = 0; d < D; ++d) fetch(ring + d * 1024);
-  int slot = 0;
   const int items = ahead.items, stride = ahead.stride;
-  for (int item = blockIdx.x * kWarps + warp; item < items; item += stride) {
+  int item = blockIdx.x * kWarps + warp;
+  Tables<DT> tables;
+  if (item < items) tables.fetch(P, Item(P, item), sub, lanes);
+  weights.fill(P, warp, lane, sub, lanes);
+  __syncthreads();
+  int slot = 0;
+  for (; item < items; item += stride) {
     const Item it(P, item);
-    const int64_t trow = (int64_t)(P.per_batch ? it.row : it.t) * P.hd;
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {
       int grp = first_of(which ? P.groups[0] : 0, it.part, P.split);
-      if (grp >= P.groups[which]) continue;
-      float ac[1][V], as[1][V], bc[1][V], bs[1][V];   // w cos, w' sin of the first half; w' cos', w sin' of the second
-      {
-        float wl[1][V], wh[1][V];
-        load_side<DT, V, 1>(wl, P.w[which], 0, P.w_dtype, sub, lanes, P.half);
-        load_side<DT, V, 1>(wh, P.w[which], P.half, P.w_dtype, sub, lanes, P.half);
-        load_side<DT, V, 1>(ac, P.cos, trow, P.t_dtype, sub, lanes, P.half);
-        load_side<DT, V, 1>(bc, P.cos, trow + P.half, P.t_dtype, sub, lanes, P.half);
-        load_side<DT, V, 1>(as, P.sin, trow, P.t_dtype, sub, lanes, P.half);
-        load_side<DT, V, 1>(bs, P.sin, trow + P.half, P.t_dtype, sub, lanes, P.half);
+      const bool some = grp < P.groups[which];
+      float ac[V], as[V], bc[V], bs[V];   // w cos, w' sin of the first half; w' cos', w sin' of the second
+      if (some) {
+        float wl[V], wh[V];
+        smem_get(wl, smem_at(&weights.w[which][0][0][lane]));
+        smem_get(wh, smem_at(&weights.w[which][1][0][lane]));
+        tables.get(ac, 0, P, sub, lanes);
+        tables.get(bc, 1, P, sub, lanes);
+        tables.get(as, 2, P, sub, lanes);
+        tables.get(bs, 3, P, sub, lanes);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          ac[0][j] *= wl[0][j];
-          as[0][j] *= wh[0][j];
-          bc[0][j] *= wh[0][j];
-          bs[0][j] *= wl[0][j];
+          ac[j] *= wl[j];
+          as[j] *= wh[j];
+          bc[j] *= wh[j];
+          bs[j] *= wl[j];
         }
       }
+      if (which && item + stride < items) tables.fetch(P, Item(P, item + stride), sub, lanes);
+      if (!some) continue;
       const int hstep = per_warp * P.split, heads = P.heads[which];
       int head = grp * per_warp + mine;
       T* o = it.at(static_cast<T*>(P.out[which]), P.os[which], head) + sub * V;
@@ -535,8 +581,8 @@ __global__ void __launch_bounds__(32 * kWarps, kFwdBlocks) qk_forward_ring_kerne
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float xl = lo.at(0, j), xh = hi.at(0, j);
-          ol[0][j] = n * fmaf(xl, ac[0][j], -xh * as[0][j]);
-          oh[0][j] = n * fmaf(xh, bc[0][j], xl * bs[0][j]);
+          ol[0][j] = n * fmaf(xl, ac[j], -xh * as[j]);
+          oh[0][j] = n * fmaf(xh, bc[j], xl * bs[j]);
         }
         if (on) {
           store_piece<DT, V, 1>(o, ol, 0, 1, V);
@@ -556,7 +602,7 @@ template <int DT> struct BwdShared {
   static constexpr int kV = DT == ZT_F32 ? 4 : 8;
   uint4 ring[kBwdWarps][kBwdRing][4][32];
   float table[kBwdWarps][4][kV / 4][32][4];   // cos, cos', sin, sin' of the warp's position
-  float weight[2][2][kV / 4][32][4];          // of q and k, both halves
+  Weights<DT> weights;
 };
 
 template <int DT, int LANES>
@@ -569,7 +615,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_backward_ring_k
   const int lanes = LANES > 0 ? LANES : P.lanes, per_warp = 32 / lanes;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, sub = lane & (lanes - 1), mine = lane / lanes;
   const uint32_t ring = smem_at(&S.ring[warp][0][0][lane]);   // a step's slot is 2048 bytes
-  const uint32_t table = smem_at(&S.table[warp][0][0][lane]), weight = smem_at(&S.weight[0][0][0][lane]);
+  const uint32_t table = smem_at(&S.table[warp][0][0][lane]), weight = smem_at(&S.weights.w[0][0][0][lane]);
   const bool in = sub * V < P.half;
   float dl[2][1][V], dh[2][1][V];
 #pragma unroll
@@ -596,23 +642,22 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_backward_ring_k
   };
 #pragma unroll 1
   for (int d = 0; d < D; ++d) fetch(ring + d * 2048);
-  if (warp < 4) {   // q lo, q hi, k lo, k hi
-    float w[1][V];
-    load_side<DT, V, 1>(w, P.w[warp / 2], (warp & 1) * P.half, P.w_dtype, sub, lanes, P.half);
-    smem_put(weight + warp * kSide, w[0]);
-  }
+  const int items = ahead.items, stride = ahead.stride;
+  int item = blockIdx.x * kBwdWarps + warp;
+  Tables<DT> tables;
+  if (item < items) tables.fetch(P, Item(P, item), sub, lanes);
+  if (warp < 4) S.weights.fill(P, warp, lane, sub, lanes);
   __syncthreads();
   int slot = 0;
-  const int items = ahead.items, stride = ahead.stride;
-  for (int item = blockIdx.x * kBwdWarps + warp; item < items; item += stride) {
+  for (; item < items; item += stride) {
     const Item it(P, item);
-    const int64_t trow = (int64_t)(P.per_batch ? it.row : it.t) * P.hd;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float v[1][V];
-      load_side<DT, V, 1>(v, i < 2 ? P.cos : P.sin, trow + (i & 1) * P.half, P.t_dtype, sub, lanes, P.half);
-      smem_put(table + i * kSide, v[0]);
+      float v[V];
+      tables.get(v, i, P, sub, lanes);
+      smem_put(table + i * kSide, v);
     }
+    if (item + stride < items) tables.fetch(P, Item(P, item + stride), sub, lanes);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       int grp = first_of(which ? P.groups[0] : 0, it.part, P.split);
