@@ -1,7 +1,7 @@
 // Fused linear distillation: the lm_head GEMM and the loss against a teacher's top logits
 // in one tcgen05 kernel, so no logit reaches HBM.
 //
-//   z[r, v] = X[r, :] . W[v, :]   (fp32 accumulate, not rounded)
+//   z[r, v] = X[r, :] . W[v, :]   (fp32, not rounded)
 //   lse[r] = log sum_v exp(z[r, v] / T),
 //   loss[r] = T^2 sum_k p_k (log p_k - z[r, i_k] / T + lse[r]),  p = softmax(t_k / T)
 //
@@ -11,12 +11,16 @@
 // 2. linear_distill_kernel on CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles, K-block
 //    64, 6 TMA stages, accumulators double-buffered in tensor memory), scheduled like the
 //    cross-entropy GEMM: the vocabulary cut into splits of a few tiles, row blocks fastest,
-//    so that the pairs in flight share W tiles in L2. An epilogue thread owns an accumulator
-//    row; beside the online (max, sum) it follows its row's sorted list through the tiles.
-//    A listed logit is fetched by a one-column load of tensor memory at that column (the
-//    column is the same for the warp's 32 rows, so a warp makes one such load per listed
-//    (row, token) of its rows and tile: about four at 64 entries of 128256 tokens).
-// 3. combine_kernel: a row's sums over the splits, then its list.
+//    so that the pairs in flight share W tiles in L2. The tensor cores truncate as they
+//    accumulate: over a K of 2048 that alone puts the loss 1.8e-6 off, over 4096 3.6e-6. So an
+//    accumulator takes 1024 of K, and the epilogue threads add these up in registers, rounding
+//    to nearest: 0.9e-6 at any K, for 1.5% of the time (512 of K: 0.4e-6 for 6%).
+//    An epilogue thread owns half an accumulator row, 128 columns; two warps share 32 rows.
+//    The first of them also follows its rows' sorted lists through the tiles: a listed logit is
+//    fetched by a one-column load of tensor memory at that column (the column is the same
+//    for the warp's 32 rows, so a warp makes at most one such load per listed token of its
+//    rows and tile: about four at 64 entries of 128256 tokens), a part for each 1024 of K.
+// 3. combine_kernel: a row's sums over the splits, then its list's logits from their parts.
 // Every mbarrier wait is bounded; on expiry the kernel records an error
 // (zt_linear_distill_take_error), drains its own copies and MMAs and frees its tensor memory.
 #include <math.h>
@@ -29,7 +33,9 @@ namespace {
 using namespace zt::tc;
 using namespace zt::distill;
 
-constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA (leader), warps 2-5 epilogue
+constexpr int kThreads = 320;  // warp 0 TMA, warp 1 MMA (leader), warps 2-9 epilogue
+constexpr int kEpilogueWarps = 8;
+constexpr int kChunk = 16;     // K-blocks of one accumulator: 1024 of K
 constexpr int kStages = 6;
 constexpr uint32_t kHalfRows = 128;
 constexpr uint32_t kStageA = kHalfRows * kBK * 2;  // 16 KB of X
@@ -50,11 +56,11 @@ struct Params {
   int32_t* status;     // [rows]
   int32_t* idx;        // [rows][top] tokens in rising order, INT32_MAX behind the last with mass
   float* lp;           // [rows][top] log2 p in that order
-  float* z;            // [rows][top] logits in that order
-  float2* partials;    // [n_splits][rows_pad] (m, s)
+  float* z;            // [n_chunks][rows][top] logits in that order, a part for each chunk of K
+  float2* partials;    // [2 n_splits][rows_pad] (m, s), of both halves of a split's tiles
   float* loss;
   float* lse;
-  int32_t rows, vocab, top, k_blocks;
+  int32_t rows, vocab, top, k_blocks, n_chunks;
   int32_t m_tiles, n_tiles, split_tiles, n_splits, rows_pad;
   float c, temperature;
   int32_t stall_loads;    // test hook: the loader issues no copies
@@ -97,6 +103,16 @@ __device__ __forceinline__ void item_range(const Params& P, int item, int& mt, i
   nt1 = min(nt0 + P.split_tiles, P.n_tiles);
 }
 
+// 32 lanes x 16 consecutive fp32 columns of tensor memory (lane = thread of the warp).
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
@@ -123,7 +139,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&accf[b], 1); mbar_init(&acce[b], 2 * 4); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&accf[b], 1); mbar_init(&acce[b], 2 * kEpilogueWarps); }
     mbar_init(drain, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -181,32 +197,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int item = cid; ok && item < n_items; item += ncl) {
         int mt, split, nt0, nt1;
         item_range(P, item, mt, split, nt0, nt1);
-        for (int nt = nt0; ok && nt < nt1; ++nt, ++tcount) {
-          const uint32_t b = tcount & 1;
-          if (!mbar_wait_pair(&acce[b], ((tcount >> 1) & 1) ^ 1, abort, peer_abort, &g_distill_error, 2, P.wait_cycles)) {
-            ok = false;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t tmem_d = tmem_base + b * kTile;
-          for (int kb = 0; kb < P.k_blocks; ++kb, ++it) {
-            const int s = it % kStages;
-            if (!mbar_wait_pair(&full[s], (it / kStages) & 1, abort, peer_abort, &g_distill_error, 3, P.wait_cycles)) {
+        for (int nt = nt0; ok && nt < nt1; ++nt) {
+          for (int k0 = 0; ok && k0 < P.k_blocks; k0 += kChunk, ++tcount) {
+            const uint32_t b = tcount & 1;
+            if (!mbar_wait_pair(&acce[b], ((tcount >> 1) & 1) ^ 1, abort, peer_abort, &g_distill_error, 2, P.wait_cycles)) {
               ok = false;
               break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t sa = smem_u32(stage_base + s * kStageBytes);
-            const uint32_t sb = sa + kStageA;
+            const uint32_t tmem_d = tmem_base + b * kTile;
+            const int k1 = min(k0 + kChunk, P.k_blocks);
+            for (int kb = k0; kb < k1; ++kb, ++it) {
+              const int s = it % kStages;
+              if (!mbar_wait_pair(&full[s], (it / kStages) & 1, abort, peer_abort, &g_distill_error, 3, P.wait_cycles)) {
+                ok = false;
+                break;
+              }
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              const uint32_t sa = smem_u32(stage_base + s * kStageBytes);
+              const uint32_t sb = sa + kStageA;
 #pragma unroll
-            for (int k = 0; k < kBK / kUmmaK; ++k)
-              umma_bf16_pair<kIdesc>(tmem_d, umma_desc(sa + k * kUmmaK * 2), umma_desc(sb + k * kUmmaK * 2),
-                                     (kb | k) != 0);
-            issued = true;
-            umma_commit_pair(&empty[s]);  // stage s is free in both CTAs once these MMAs have read it
+              for (int k = 0; k < kBK / kUmmaK; ++k)
+                umma_bf16_pair<kIdesc>(tmem_d, umma_desc(sa + k * kUmmaK * 2), umma_desc(sb + k * kUmmaK * 2),
+                                       kb != k0 || k != 0);
+              issued = true;
+              umma_commit_pair(&empty[s]);  // stage s is free in both CTAs once these MMAs have read it
+            }
+            if (!ok) break;
+            umma_commit_pair(&accf[b]);  // accumulator b is complete in both CTAs
           }
-          if (!ok) break;
-          umma_commit_pair(&accf[b]);  // accumulator b is complete in both CTAs
         }
       }
       if (issued) {  // wait (bounded) for every MMA issued by this thread before exit
@@ -214,8 +233,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         mbar_drain(drain, 0);
       }
     }
-  } else {  // ---- epilogue: warps 2..5 of both CTAs; each thread owns one accumulator row
-    const int q = warp & 3;
+  } else {  // ---- epilogue: warps 2..9 of both CTAs; each thread owns half an accumulator row
+    const int q = warp & 3, half = (warp - 2) >> 2;
     const int row_local = q * 32 + lane;
     const uint32_t leader_acce0 = peer_addr(&acce[0], 0), leader_acce1 = peer_addr(&acce[1], 0);
     uint32_t tcount = 0;
@@ -227,8 +246,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // the row's list from this split's first column on: its place, its next two tokens
       const int32_t* list = P.idx + (int64_t)row * P.top;
       int pos = P.top, next = INT32_MAX, after = INT32_MAX;
-      if (row < P.rows) {
-        int lo = 0, hi = P.top;
+      if (half == 0 && row < P.rows) {
+        int lo = 0, hi = nt0 > 0 ? P.top : 0;
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
           if (list[mid] < nt0 * kTile) lo = mid + 1;
@@ -239,46 +258,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (pos + 1 < P.top) after = list[pos + 1];
       }
       Stat st{-INFINITY, 0.f};
-      for (int nt = nt0; nt < nt1; ++nt, ++tcount) {
-        const uint32_t b = tcount & 1;
-        int okw = 1;
-        if (lane == 0) okw = mbar_wait_pair(&accf[b], (tcount >> 1) & 1, abort, peer_abort, &g_distill_error, 4, P.wait_cycles) ? 1 : 0;
-        okw = __shfl_sync(0xffffffffu, okw, 0);
-        if (!okw) { ok = false; break; }
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + b * kTile;
+      for (int nt = nt0; ok && nt < nt1; ++nt) {
         const int tile0 = nt * kTile;
-        for (;;) {  // the listed columns of this tile, one column of the warp's rows at a time
-          const int col = __reduce_min_sync(0xffffffffu, next);   // each column once, in order
-          if (col >= tile0 + kTile) break;
-          const float v = tmem_ld1(acc + (uint32_t)(col - tile0));
-          if (next == col) {
-            P.z[(int64_t)row * P.top + pos] = v;
-            ++pos;
-            next = after;
-            after = pos + 1 < P.top ? list[pos + 1] : INT32_MAX;
-          }
+        float sum[kTile / 2];
+        const int pos0 = pos, next0 = next;
+        for (int ch = 0; ch < P.n_chunks; ++ch, ++tcount) {
+          const uint32_t b = tcount & 1;
+          int okw = 1;
+          if (lane == 0) okw = mbar_wait_pair(&accf[b], (tcount >> 1) & 1, abort, peer_abort, &g_distill_error, 4, P.wait_cycles) ? 1 : 0;
+          okw = __shfl_sync(0xffffffffu, okw, 0);
+          if (!okw) { ok = false; break; }
           __syncwarp();
-        }
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld32(acc + (uint32_t)c0, r);
-          float v[32];
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + b * kTile;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          if (tile0 + c0 + 32 > P.vocab) {  // the padded columns of the last tile
+          for (int c0 = 0; c0 < kTile / 2; c0 += 16) {
+            uint32_t r[16];
+            tmem_ld16(acc + (uint32_t)(half * (kTile / 2) + c0), r);
+            if (ch == 0) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (tile0 + c0 + j >= P.vocab) v[j] = -INFINITY;
+              for (int j = 0; j < 16; ++j) sum[c0 + j] = __uint_as_float(r[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[c0 + j] += __uint_as_float(r[j]);
+            }
           }
-          absorb(st, v, P.c);
+          if (half == 0) {
+            pos = pos0;
+            next = next0;
+            bool fresh = true;
+            float* z = P.z + ((int64_t)ch * P.rows + row) * P.top;
+            for (;;) {  // the listed columns of this tile, one column of the warp's rows at a time
+              const int col = __reduce_min_sync(0xffffffffu, next);   // each column once, in order
+              if (col >= tile0 + kTile) break;
+              const float v = tmem_ld1(acc + (uint32_t)(col - tile0));
+              while (next == col) {   // again where the token stands in the list several times
+                z[pos] = v;
+                ++pos;
+                // `after` is loaded once a tile: a load here would hold up the whole warp at its
+                // next turn, and a row seldom has two tokens in a tile
+                next = fresh ? after : pos < P.top ? list[pos] : INT32_MAX;
+                fresh = false;
+              }
+              __syncwarp();
+            }
+          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(b ? leader_acce1 : leader_acce0);  // accumulator b may be overwritten
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(b ? leader_acce1 : leader_acce0);  // accumulator b may be overwritten
+        if (!ok) break;
+        if (pos != pos0) after = pos + 1 < P.top ? list[pos + 1] : INT32_MAX;
+        const int col0 = tile0 + half * (kTile / 2);
+        if (col0 + kTile / 2 > P.vocab) {  // the padded columns of the last tile
+#pragma unroll
+          for (int j = 0; j < kTile / 2; ++j)
+            if (col0 + j >= P.vocab) sum[j] = -INFINITY;
+        }
+        absorb(st, sum, P.c);
       }
-      if (ok && row < P.rows) P.partials[(size_t)split * P.rows_pad + row] = make_float2(st.m, st.s);
+      if (ok && row < P.rows) P.partials[(size_t)(2 * split + half) * P.rows_pad + row] = make_float2(st.m, st.s);
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -301,6 +340,13 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
   const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
   const int64_t row = row0 + warp;
   constexpr int kHeld = 4;   // list entries of a lane loaded ahead
+  const int64_t part_stride = (int64_t)P.rows * P.top;
+  auto logit = [&](int64_t at) {   // the parts in order
+    float v = 0.f;
+#pragma unroll 4
+    for (int ch = 0; ch < P.n_chunks; ++ch) v += __ldg(P.z + ch * part_stride + at);
+    return v;
+  };
   int32_t idx[kHeld], status = kNoTeacher;
   float lp[kHeld], z[kHeld];
 #pragma unroll
@@ -310,13 +356,13 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
       const int64_t at = row * P.top + lane + 32 * e;
       idx[e] = __ldg(P.idx + at);
       lp[e] = __ldg(P.lp + at);
-      z[e] = __ldg(P.z + at);   // not written where idx is INT32_MAX, and then not looked at
+      z[e] = logit(at);   // not written where idx is INT32_MAX, and then not looked at
     }
   }
   if (row < P.rows) status = __ldg(P.status + row);
   Stat st{-INFINITY, 0.f};
 #pragma unroll 4
-  for (int sp = tid / kCombineRows; sp < P.n_splits; sp += 32 * kListWarps / kCombineRows) {   // rows_pad covers the block
+  for (int sp = tid / kCombineRows; sp < 2 * P.n_splits; sp += 32 * kListWarps / kCombineRows) {   // rows_pad covers the block
     const float2 o = __ldg(P.partials + (size_t)sp * P.rows_pad + row0 + tid % kCombineRows);
     st = merge(st, Stat{o.x, o.y}, P.c);
   }
@@ -343,7 +389,7 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
     if (idx[e] != INT32_MAX) add(lp[e], z[e]);
   for (int k = lane + 32 * kHeld; k < P.top; k += 32) {
     const int64_t at = row * P.top + k;
-    if (P.idx[at] != INT32_MAX) add(P.lp[at], P.z[at]);
+    if (P.idx[at] != INT32_MAX) add(P.lp[at], logit(at));
   }
   a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
   if (lane == 0) {
@@ -431,13 +477,15 @@ struct Layout {
   size_t idx, lp, z, status, total;
 };
 
-Layout layout(const Split& sp, int64_t rows, int32_t top) {
-  const size_t entries = up256((size_t)rows * (size_t)top * 4);
+int32_t chunks_of(int64_t k) { return (int32_t)((k / kBK + kChunk - 1) / kChunk); }
+
+Layout layout(const Split& sp, int64_t rows, int32_t top, int32_t n_chunks) {
+  const size_t entries = (size_t)rows * (size_t)top * 4;
   Layout L;
-  L.idx = up256(sizeof(float2) * (size_t)sp.n_splits * (size_t)sp.rows_pad);
-  L.lp = L.idx + entries;
-  L.z = L.lp + entries;
-  L.status = L.z + entries;
+  L.idx = up256(2 * sizeof(float2) * (size_t)sp.n_splits * (size_t)sp.rows_pad);
+  L.lp = L.idx + up256(entries);
+  L.z = L.lp + up256(entries);
+  L.status = L.z + up256(entries * (size_t)n_chunks);
   L.total = L.status + up256((size_t)rows * 4);
   return L;
 }
@@ -451,7 +499,7 @@ size_t zt_linear_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k,
   if (check_shape(rows, vocab, k, top)) return 0;
   int dev = 0, pairs = 0;
   if (device_pairs(&dev, &pairs)) return 0;
-  return layout(choose_split(rows, vocab, pairs), rows, top).total;
+  return layout(choose_split(rows, vocab, pairs), rows, top, chunks_of(k)).total;
 }
 
 int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
@@ -468,7 +516,7 @@ int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
   int dev = 0, pairs = 0;
   if (int rc = device_pairs(&dev, &pairs)) return rc;
   const Split sp = choose_split(a->rows, a->vocab, pairs);
-  const Layout L = layout(sp, a->rows, a->top);
+  const Layout L = layout(sp, a->rows, a->top, chunks_of(a->k));
   if (a->workspace_bytes < L.total) return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: workspace too small");
   EncodeFn enc = nullptr;
   if (int rc = get_encode(&enc, "zt_linear_distill")) return rc;
@@ -490,6 +538,7 @@ int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
   P.vocab = (int32_t)a->vocab;
   P.top = a->top;
   P.k_blocks = (int32_t)(a->k / kBK);
+  P.n_chunks = chunks_of(a->k);
   P.m_tiles = sp.m_tiles;
   P.n_tiles = sp.n_tiles;
   P.split_tiles = sp.split_tiles;
