@@ -158,15 +158,17 @@ template <int DT> __device__ __forceinline__ Span<DT> span_of(const RowsParams& 
 
 // Step g of S threads, U vectors each, over a span; 2^((-inf - m) c) = 0 stands in for what is beyond.
 template <int DT, int S, int U> __device__ __forceinline__ void load_step(uint4 (&u)[U], const Span<DT>& sp, int g, bool again) {
-  const uint4* v = sp.vec();
+  const int i = threadIdx.x + g * (U * S);
+  const uint4* v = sp.vec() + i;
+  if ((g + 1) * (U * S) <= sp.n_vec) {
 #pragma unroll
-  for (int j = 0; j < U; ++j) {
-    const int i = threadIdx.x + (g * U + j) * S;
-    if (i < sp.n_vec) {
-      u[j] = again ? __ldcg(v + i) : __ldcs(v + i);
-    } else {
-      const uint32_t w = DT == ZT_F32 ? 0xff800000u : DT == ZT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+    for (int j = 0; j < U; ++j) u[j] = again ? __ldcg(v + j * S) : __ldcs(v + j * S);
+  } else {
+    const uint32_t w = DT == ZT_F32 ? 0xff800000u : DT == ZT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
       u[j] = make_uint4(w, w, w, w);
+      if (i + j * S < sp.n_vec) u[j] = again ? __ldcg(v + j * S) : __ldcs(v + j * S);
     }
   }
 }
@@ -356,7 +358,7 @@ template <int DT> struct Dense {
 
   __device__ __forceinline__ Dense(const Stat& st, float A, float c) : base(st.m, c), a(A / st.s), k(0.f), sign(0), fold(false) {
     if (DT != ZT_F32) {
-      if (a < 0.f) sign = 0x80008000u;
+      if (a < 0.f) sign = 0x80008000u;   // the paired sign bits
       a = fabsf(a);
       k = log2f(a) - base.mc;
       fold = fabsf(base.mc) <= 64.f;
@@ -366,10 +368,10 @@ template <int DT> struct Dense {
     const float v = fold ? ex2(__fmaf_rn(El<DT>::to(z), c, k)) : a * ex2(base.rel(El<DT>::to(z), c));
     return El<DT>::from(sign ? -v : v);
   }
-  __device__ __forceinline__ uint4 vec(const uint4& u, float c) const {
+  template <bool FOLD> __device__ __forceinline__ uint4 vec(const uint4& u, float c) const {
     float f[V];
     El<DT>::unpack(u, f);
-    if (DT != ZT_F32 && fold) {
+    if (FOLD) {
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] = ex2(__fmaf_rn(f[i], c, k));
     } else if (!base.far()) {
@@ -387,34 +389,45 @@ template <int DT> struct Dense {
   }
 };
 
-// The stream threads' part of a row's gradient over a span; `u` holds step 0, loaded before the
-// caller waited for anything, and each step is loaded before the one before it is written.
-// out has its own 16-byte phase.
-template <int DT, int S, int U>
-__device__ __forceinline__ void write_span(uint4 (&u)[U], const Span<DT>& sp, typename El<DT>::T* out, const Dense<DT>& D, float c) {
+// The vectors of a row's gradient over a span; `u` holds step 0, loaded before the caller waited
+// for anything, and each step is loaded before the one before it is written. SAME: the gradient's
+// vectors are as aligned as the logits'.
+template <int DT, int S, int U, bool FOLD, bool SAME>
+__device__ __forceinline__ void write_vecs(uint4 (&u)[U], const Span<DT>& sp, typename El<DT>::T* out, const Dense<DT>& D, float c) {
   using T = typename El<DT>::T;
   constexpr int V = El<DT>::kVec;
-  const int n = steps_of<DT, S, U>(sp), tid = threadIdx.x;
-  const bool same = ((uintptr_t)(out + sp.body) & 15) == 0;
+  const int n = steps_of<DT, S, U>(sp);
+  int i = threadIdx.x;
+  T* o = out + sp.body + i * V;
   uint4 next[U];
   for (int g = 0; g < n; ++g) {
     if (g + 1 < n) load_step<DT, S, U>(next, sp, g + 1, false);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int i = tid + (g * U + j) * S;
-      if (i < sp.n_vec) {
-        const uint4 r = D.vec(u[j], c);
-        if (same) {
-          __stcs(reinterpret_cast<uint4*>(out + sp.body) + i, r);
+      const uint4 r = D.template vec<FOLD>(u[j], c);
+      if (i + j * S < sp.n_vec) {
+        if (SAME) {
+          __stcs(reinterpret_cast<uint4*>(o) + j * S, r);
         } else {   // an element at a time; in place this cannot be
           const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-          for (int k = 0; k < V; ++k) out[sp.body + i * V + k] = e[k];
+          for (int k = 0; k < V; ++k) o[j * S * V + k] = e[k];
         }
       }
       u[j] = next[j];
     }
+    i += U * S;
+    o += U * S * V;
   }
+}
+
+// The stream threads' part of a row's gradient over a span. out has its own 16-byte phase.
+template <int DT, int S, int U>
+__device__ __forceinline__ void write_span(uint4 (&u)[U], const Span<DT>& sp, typename El<DT>::T* out, const Dense<DT>& D, float c) {
+  const int tid = threadIdx.x;
+  if (((uintptr_t)(out + sp.body) & 15) != 0) write_vecs<DT, S, U, false, false>(u, sp, out, D, c);
+  else if (DT != ZT_F32 && D.fold) write_vecs<DT, S, U, true, true>(u, sp, out, D, c);
+  else write_vecs<DT, S, U, false, true>(u, sp, out, D, c);
   if (tid < sp.body - sp.lo) out[sp.lo + tid] = D.one(sp.row[sp.lo + tid], c);
   if (tid < sp.hi - sp.tail()) out[sp.tail() + tid] = D.one(sp.row[sp.tail() + tid], c);
 }
