@@ -577,6 +577,127 @@ def test_criterion_zeroth_and_first_order():
     assert math.isfinite(float(out["loss"])) and not torch.equal(before, w.detach())
 
 
+def test_differentiable_once():
+    from zotitan_b200 import kernels as K
+    z, idx, val = make(4, 300, 5, torch.float32, seed=14)
+    leaf = z.detach().requires_grad_()
+    one = torch.ones(4, device="cuda")
+    plain, = torch.autograd.grad(K.distill_rows(leaf, idx, val)[0], leaf, one)
+    grad, = torch.autograd.grad(K.distill_rows(leaf, idx, val)[0], leaf, one, create_graph=True)
+    assert torch.equal(grad, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(grad.sum(), leaf)
+
+
+def test_padded_batch():
+    """Most rows without a teacher, their logits NaN: zeros there, the others as on their own."""
+    from zotitan_b200 import kernels as K
+    for dt, vocab, shift in (("bf16", 30001, 0), ("f32", 9001, 1), ("f16", 5003, 3)):
+        z, idx, val = make(400, vocab, 8, DTYPES[dt], seed=15, empty=False, shift=shift)
+        w = torch.rand(400, device="cuda")
+        keep = torch.arange(400, device="cuda") % 5 == 2
+        alone = K.distill_rows_grad(z[keep].contiguous(), idx[keep], val[keep], w[keep])
+        z[~keep], idx[~keep] = math.nan, -1
+        leaf = z.detach().requires_grad_()
+        loss, lse = K.distill_rows(leaf, idx, val)
+        grad, = torch.autograd.grad(loss, leaf, w)
+        one = K.distill_rows_grad(z, idx, val, w)
+        for lo, ls, gr in ((loss, lse, grad), one):
+            assert not lo[~keep].any() and not ls[~keep].any() and not gr[~keep].any()
+        e = Exact(z[keep], idx[keep], val[keep], 1.0)
+        want, tol = e.grad(w[keep])
+        close(grad[keep], want, tol, DTYPES[dt])
+        close(one[2][keep], want, tol, DTYPES[dt])
+        close(one[0][keep], e.loss, e.tol_loss, torch.float32)
+        close(alone[0], e.loss, e.tol_loss, torch.float32)
+
+
+def test_large_biases():
+    """Logits far from zero: the common part cancels in loss and gradient (16-bit logits that far
+    apart are exact inputs all the same)."""
+    from zotitan_b200 import kernels as K
+    for dt, shift in (("f32", 3000.0), ("f32", 726817.0), ("f32", 1e7), ("f32", -1e20), ("f16", -2000.0), ("bf16", 1e4), ("f32", 2e30)):
+        dtype = DTYPES[dt]
+        z, idx, val = make(6, 2000, 9, dtype, seed=16, empty=False)
+        z = (z.float() + shift).to(dtype)
+        e = Exact(z, idx, val, 1.0)
+        leaf = z.detach().requires_grad_()
+        loss, lse = K.distill_rows(leaf, idx, val)
+        # mc = round(m log2 e) is the same for every term; its own rounding shows in lse alone
+        close(loss.detach(), e.loss, e.tol_loss, torch.float32)
+        close(lse.detach(), e.lse, e.tol_lse, torch.float32)
+        g = torch.full((6,), 64.0, device="cuda")
+        want, tol = e.grad(g)
+        got, = torch.autograd.grad(loss, leaf, g)
+        close(got, want, tol, dtype)
+        close(K.distill_rows_grad(z, idx, val, g)[2], want, tol, dtype)
+
+
+def test_generation_with_a_cache():
+    """The fused attention with a key-value cache: a prompt, then a token, against the whole
+    sequence at once."""
+    from zotitan_b200.llama_fused import fuse_llama
+    m = model_with_head_norms(seed=4)
+    ids = torch.randint(0, 1000, (2, 17), device="cuda")
+    with torch.inference_mode():
+        plain = m(input_ids=ids).logits[:, -1].float()
+        fuse_llama(m)
+        whole = m(input_ids=ids).logits[:, -1].float()
+        first = m(input_ids=ids[:, :-1], use_cache=True)
+        last = m(input_ids=ids[:, -1:], past_key_values=first.past_key_values, use_cache=True).logits[:, -1].float()
+    scale = float(plain.square().mean().sqrt())
+    for got in (whole, last):
+        assert float((got - plain).square().mean().sqrt()) <= 0.05 * scale
+
+
+def test_hooked_head_norms_are_left_alone():
+    from zotitan_b200.llama_fused import fuse_llama
+    m = model_with_head_norms(seed=5, layers=1)
+    fuse_llama(m)
+    seen = []
+    m.model.layers[0].self_attn.q_norm.register_forward_hook(lambda *_: seen.append(1))
+    with torch.inference_mode():
+        m(input_ids=torch.randint(0, 1000, (1, 8), device="cuda"))
+    assert seen
+
+
+FIRST = """
+import torch
+from zotitan_b200 import kernels as K
+g = torch.Generator(device="cuda").manual_seed(0)
+z = torch.randn(40, 3000, device="cuda", generator=g).bfloat16()
+val, idx = torch.topk(z.float(), 8, dim=1)
+x, w = torch.randn(40, 64, device="cuda", generator=g).bfloat16(), torch.randn(3000, 64, device="cuda", generator=g).bfloat16()
+q, k = torch.randn(2, 9, 4, 64, device="cuda", generator=g).bfloat16(), torch.randn(2, 9, 2, 64, device="cuda", generator=g).bfloat16()
+wt, tab = torch.ones(64, device="cuda").bfloat16(), torch.rand(9, 64, device="cuda", generator=g).bfloat16()
+weight = torch.ones(40, device="cuda")
+
+def step():
+    a, b = z.detach().requires_grad_(), q.detach().requires_grad_()
+    loss, lse = K.distill_rows(a, idx, val)
+    out = [loss, lse, *torch.autograd.grad(loss, a, weight), *K.distill_rows_grad(z, idx, val, weight), *K.linear_distill(x, w, idx, val)]
+    rot = K.qk_norm_rope(b, k, wt, wt, tab, tab)
+    return [t.detach() for t in (*out, *rot, *torch.autograd.grad(rot[0], b, torch.ones_like(rot[0])))]
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(p, r) for p, r in zip(out, step()))
+print("captured first")
+"""
+
+
+def test_captured_before_any_other_call():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
 def test_refusals():
     from zotitan_b200 import kernels as K
     z, idx, val = make(8, 500, 6, torch.bfloat16, seed=12)

@@ -299,3 +299,53 @@ def test_refusals():
         K.qk_norm_rope_(q[:1].expand(2, -1, -1, -1), k, wq, wk, cos, sin)
     with pytest.raises(ValueError, match="differentiable"):
         K.qk_norm_rope_(q, k, wq.detach().requires_grad_(), wk, cos, sin)
+
+
+def test_far_elements():
+    """Positions whose elements lie beyond 2^31, read, written in place and differentiated."""
+    from zotitan_b200 import kernels as K
+    step = (1 << 30) + 64
+    q, k, wq, wk, cos, sin, gq, gk = make(1, 3, 4, 2, 64, torch.bfloat16, seed=12)
+    store = torch.empty(3 * step, dtype=torch.bfloat16, device="cuda")
+    fq = store.as_strided((1, 3, 4, 64), (0, step, 64, 1))
+    fk = store.as_strided((1, 3, 2, 64), (0, step, 64, 1), 4096)
+    fq.copy_(q), fk.copy_(k)
+    want = K.qk_norm_rope(q, k, wq, wk, cos, sin)
+    got = K.qk_norm_rope(fq, fk, wq, wk, cos, sin)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    a, b = q.detach().requires_grad_(), fq.detach().requires_grad_()
+    grads = [torch.autograd.grad(K.qk_norm_rope(x, y, wq, wk, cos, sin)[0], x, gq)[0] for x, y in ((a, k), (b, fk))]
+    assert torch.equal(*grads)
+    K.qk_norm_rope_(fq, fk, wq, wk, cos, sin)
+    assert torch.equal(fq, want[0]) and torch.equal(fk, want[1])
+
+
+def test_differentiable_once():
+    from zotitan_b200 import kernels as K
+    q, k, wq, wk, cos, sin, gq, _ = make(1, 5, 2, 1, 64, torch.float32, seed=13)
+    leaf = q.detach().requires_grad_()
+    plain, = torch.autograd.grad(K.qk_norm_rope(leaf, k, wq, wk, cos, sin)[0], leaf, gq)
+    dq, = torch.autograd.grad(K.qk_norm_rope(leaf, k, wq, wk, cos, sin)[0], leaf, gq, create_graph=True)
+    assert torch.equal(dq, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), leaf)
+
+
+def test_two_at_once():
+    """The same weights and tables on two streams at the same time."""
+    from zotitan_b200 import kernels as K
+    cases = [make(4, 64, 8, 2, 128, torch.bfloat16, seed=s) for s in (14, 15)]
+    want = []
+    for q, k, wq, wk, cos, sin, gq, gk in cases:
+        leaves = [t.detach().requires_grad_() for t in (q, k, wq, wk)]
+        want.append(torch.autograd.grad(K.qk_norm_rope(*leaves, cos, sin), leaves, (gq, gk)))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (q, k, wq, wk, cos, sin, gq, gk) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                leaves = [t.detach().requires_grad_() for t in (q, k, wq, wk)]
+                got[i].append(torch.autograd.grad(K.qk_norm_rope(*leaves, cos, sin), leaves, (gq, gk)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in (0, 1) for g in got[i] for a, b in zip(g, want[i]))

@@ -432,9 +432,16 @@ __device__ __forceinline__ void write_span(uint4 (&u)[U], const Span<DT>& sp, ty
   if (tid < sp.hi - sp.tail()) out[sp.tail() + tid] = D.one(sp.row[sp.tail() + tid], c);
 }
 
+// The gradient of a row without a teacher.
 template <int DT, int S>
-__device__ __forceinline__ void zero_span(const Span<DT>& sp, typename El<DT>::T* out) {
-  for (int i = sp.lo + threadIdx.x; i < sp.hi; i += S) out[i] = El<DT>::from(0.f);
+__device__ __forceinline__ void zero_span(typename El<DT>::T* out, int32_t lo, int32_t hi) {
+  const Span<DT> o(out, lo, hi);
+  const int tid = threadIdx.x;
+  const typename El<DT>::T zero = El<DT>::from(0.f);
+  uint4* v = reinterpret_cast<uint4*>(out + o.body);
+  for (int i = tid; i < o.n_vec; i += S) v[i] = make_uint4(0, 0, 0, 0);
+  if (tid < o.body - o.lo) out[o.lo + tid] = zero;
+  if (tid < o.hi - o.tail()) out[o.tail() + tid] = zero;
 }
 
 template <int DT>
@@ -463,7 +470,7 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backwa
   }
   if (P.grad == P.z) __syncthreads();   // in place: the listed logits are read before they are overwritten
   if (tid < S) {
-    if (none) zero_span<DT, S>(sp, out);
+    if (none) zero_span<DT, S>(out, sp.lo, sp.hi);
     else write_span<DT, S, U>(u, sp, out, Dense<DT>(st, A, P.c), P.c);
   }
   __syncthreads();
@@ -502,7 +509,7 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_grad_k
     if (part == 0) write_loss<S>(sh, P, row, st);
     list_sums(sh.list, P.list.top);   // after the loss: it takes the place of log2 p
   } else if (none) {
-    zero_span<DT, S>(sp, out);
+    zero_span<DT, S>(out, sp.lo, sp.hi);
   } else {
     write_span<DT, S, U>(u, sp, out, Dense<DT>(st, A, P.c), P.c);
   }

@@ -23,17 +23,17 @@ __device__ __forceinline__ float ex2(float x) {
 // maximum of their own some lane of a warp has a new one at almost every step, and the rescaling
 // measured a third of the instructions. A sum of 2^30 such terms stays below 2^47.
 //
-// (z - m) c is fma(z, c, -mc) with mc = round(m c): one instruction, and its rounding of m c is
-// the same for every term, so that it cancels as long as all uses of a sum take the same mc
-// (merging two sums multiplies by 2^(mc - mc'), and logs of q are relative to mc). Beyond
-// kFar, where z c may leave the range (a logit at its type's lowest value), the
-// difference is taken first: such a logit gives 2^-inf = 0, and a row of nothing else stays
-// finite.
+// (z - m) c is fma(z, c, -mc) with mc = round(m c): one instruction, and what mc's rounding takes
+// off the exponent is the same for every term, so that it cancels as long as all uses of a sum
+// take the same mc. That holds while it is small: beyond |mc| = kFar (where it may be 2^-4) the
+// difference is taken first, which is exact for z near m. So rows with a common part of
+// any size keep their softmax, a logit at its type's lowest value gives 2^-inf = 0, and a row of
+// nothing else stays finite.
 struct Stat {
   float m, s;
 };
 
-constexpr float kFar = 1e30f;
+constexpr float kFar = 1048576.f;
 constexpr float kSlack = 16.f;
 
 struct Base {
@@ -42,15 +42,21 @@ struct Base {
     m = max == -INFINITY ? 0.f : max;
     mc = __fmul_rn(m, c);
   }
-  __device__ __forceinline__ bool far() const { return fabsf(m) > kFar; }
+  __device__ __forceinline__ bool far() const { return fabsf(mc) > kFar; }
   __device__ __forceinline__ float rel(float z, float c) const { return far() ? (z - m) * c : __fmaf_rn(z, c, -mc); }
 };
 
-// The factor that takes a sum from base a to the larger b.
+// The factor that takes a sum from base a to the larger b: 2 to the difference of what the two
+// sums are relative to, mc or, far out, m c itself.
 __device__ __forceinline__ float rescale(float a, float b, float c) {
   if (a == -INFINITY) return 0.f;
-  if (fabsf(a) > kFar || fabsf(b) > kFar) return ex2((a - b) * c);
-  return ex2(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, c)));
+  const float ac = __fmul_rn(a, c), bc = __fmul_rn(b, c);
+  const bool fa = fabsf(ac) > kFar, fb = fabsf(bc) > kFar;
+  if (!fa && !fb) return ex2(__fsub_rn(ac, bc));
+  float d = (a - b) * c;
+  if (!fa) d -= __fmaf_rn(a, c, -ac);
+  if (!fb) d += __fmaf_rn(b, c, -bc);
+  return ex2(d);
 }
 
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float c) {

@@ -103,18 +103,25 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
     return self.o_proj(out.reshape(bsz, T, -1).contiguous()), weights
 
 
+def _plain_norm(m, hd: int) -> bool:
+    """A head norm as the model built it: nothing hooked onto it that the fused pass would skip."""
+    return (type(m).__name__ == "Qwen3RMSNorm" and m.weight.shape == (hd,) and not m._forward_hooks
+            and not m._forward_pre_hooks and not m._backward_hooks and not m._backward_pre_hooks)
+
+
 def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None,
                                **kwargs):
     cos, sin = position_embeddings if position_embeddings is not None else (None, None)
     hd = self.head_dim
+    dt = hidden_states.dtype
+    if not _plain_norm(self.q_norm, hd) or not _plain_norm(self.k_norm, hd):
+        return self._zt_orig_forward(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
     wq, wk = self.q_norm.weight, self.k_norm.weight
     eps = self.q_norm.variance_epsilon
-    dt = hidden_states.dtype
     if (not hidden_states.is_cuda or dt not in (torch.bfloat16, torch.float16, torch.float32) or cos is None
             or hidden_states.dim() != 3 or hidden_states.numel() == 0 or cos.dim() != 3
             or cos.shape[0] not in (1, hidden_states.shape[0]) or cos.shape[1:] != (hidden_states.shape[1], hd) or hd % 2
-            or hd > 512 or eps != self.k_norm.variance_epsilon or wq.shape != (hd,) or wk.shape != (hd,)
-            or wq.dtype != wk.dtype or wq.dtype not in (dt, torch.float32) or cos.dtype not in (dt, torch.float32)
+            or hd > 512 or eps != self.k_norm.variance_epsilon or wq.dtype != wk.dtype or wq.dtype not in (dt, torch.float32) or cos.dtype not in (dt, torch.float32)
             or torch.is_autocast_enabled("cuda")):
         return self._zt_orig_forward(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
     from transformers.models.qwen3.modeling_qwen3 import ALL_ATTENTION_FUNCTIONS, eager_attention_forward

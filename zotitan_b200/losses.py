@@ -147,7 +147,7 @@ def head_distill(hidden: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.
     where that requires grad (then the whole logits are kept, as the backward needs them);
     lse is differentiable only in that last form."""
     train_head = weight.requires_grad or (bias is not None and bias.requires_grad)
-    if torch.is_grad_enabled() and train_head:
+    if torch.is_grad_enabled() and (train_head or torch.is_autocast_enabled("cuda")):
         return K.distill_rows(F.linear(hidden, weight, bias), top_idx, top_logits, temperature)
     if torch.is_grad_enabled() and hidden.requires_grad:
         return _FrozenHeadDistill.apply(hidden, weight, bias, top_idx, top_logits, temperature, chunk_rows)
