@@ -29,6 +29,7 @@ using zt::tc::peer_addr;
 // a thread also loads its next step ahead (its registers cost warps).
 constexpr int kSumThreads = 256, kSumCtas = 6, kSumStep = 2;
 constexpr int kWriteThreads = 512, kWriteCtas = 2, kWriteStep = 4;   // backward, and loss and gradient at once
+constexpr int kRowWarps = 8;         // rows of a block where a warp takes a row
 constexpr int kMaxCluster = 8;
 
 struct RowsParams {
@@ -157,8 +158,9 @@ template <int DT> __device__ __forceinline__ Span<DT> span_of(const RowsParams& 
 }
 
 // Step g of S threads, U vectors each, over a span; 2^((-inf - m) c) = 0 stands in for what is beyond.
-template <int DT, int S, int U> __device__ __forceinline__ void load_step(uint4 (&u)[U], const Span<DT>& sp, int g, bool again) {
-  const int i = threadIdx.x + g * (U * S);
+template <int DT, int S, int U>
+__device__ __forceinline__ void load_step(uint4 (&u)[U], const Span<DT>& sp, int tid, int g, bool again) {
+  const int i = tid + g * (U * S);
   const uint4* v = sp.vec() + i;
   if ((g + 1) * (U * S) <= sp.n_vec) {
 #pragma unroll
@@ -188,16 +190,16 @@ template <int DT, int U> __device__ __forceinline__ void absorb_step(Stat& st, c
   absorb(st, f, El<DT>::max_of(u), c);
 }
 
-// A thread's share of a span's sum; gives up once the row is known to have no teacher. `again`:
-// the span will be read once more and should stay in L2.
+// Thread tid's share of a span's sum; gives up once the row is known to have no teacher (where
+// `none` is watched). `again`: the span will be read once more and should stay in L2.
 template <int DT, int S, int U>
-__device__ __forceinline__ Stat sum_span(const Span<DT>& sp, float c, const volatile int* none, bool again) {
+__device__ __forceinline__ Stat sum_span(const Span<DT>& sp, int tid, float c, const volatile int* none, bool again) {
   Stat st{-INFINITY, 0.f};
-  const int n = steps_of<DT, S, U>(sp), tid = threadIdx.x;
+  const int n = steps_of<DT, S, U>(sp);
   uint4 u[U];
   for (int g = 0; g < n; ++g) {
-    load_step<DT, S, U>(u, sp, g, again);
-    if (*none) break;
+    load_step<DT, S, U>(u, sp, tid, g, again);
+    if (none && *none) break;
     absorb_step<DT, U>(st, u, c);
   }
   if (tid < sp.body - sp.lo) {
@@ -219,7 +221,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 
 // What the CTAs of a row share, and a CTA's threads.
 template <int S> struct Shared {
-  List list;
+  unsigned long long list[kMaxTop * List::kBytes / 8];
   Stat red[S / 32];   // the warps' sums
   Stat mine, total;   // this CTA's, the row's
   int none, bad;      // no teacher: the row's logits need not be read; an index that does not exist
@@ -269,7 +271,7 @@ __device__ __forceinline__ Stat final_stat(Stat st, bool bad) {
 
 // The row's logits at the list's indices inside [lo, hi).
 template <int DT>
-__device__ __forceinline__ void gather(List& s, const typename El<DT>::T* row, int top, int32_t lo, int32_t hi) {
+__device__ __forceinline__ void gather(const List& s, const typename El<DT>::T* row, int top, int32_t lo, int32_t hi) {
 #pragma unroll 4
   for (int k = threadIdx.x & 31; k < top; k += 32) {
     const int32_t i = s.idx[k];
@@ -281,22 +283,23 @@ __device__ __forceinline__ void gather(List& s, const typename El<DT>::T* row, i
 // the teacher's probabilities.
 template <int DT, int S>
 __device__ __forceinline__ void prepare_list(Shared<S>& sh, const RowsParams& P, int64_t row, int32_t lo, int32_t hi) {
-  const Teacher t = read_list(sh.list, P.list, row);
+  const List list(sh.list, kMaxTop);
+  const Teacher t = read_list(list, P.list, row);
   if ((threadIdx.x & 31) == 0) {
     sh.bad = t.bad;
     if (!t.any) *(volatile int*)&sh.none = 1;
   }
-  gather<DT>(sh.list, static_cast<const typename El<DT>::T*>(P.z) + row * P.ld, P.list.top, lo, hi);
-  list_softmax(sh.list, P.list.top, P.c);
+  gather<DT>(list, static_cast<const typename El<DT>::T*>(P.z) + row * P.ld, P.list.top, lo, hi);
+  list_softmax(list, P.list.top, P.c);
 }
 
 // and after: loss, lse and what the backward needs.
-template <int S> __device__ __forceinline__ void write_loss(const Shared<S>& sh, const RowsParams& P, int64_t row, Stat st) {
-  const float loss = list_loss(sh.list, P.list.top, st, P.c, P.temperature);
+__device__ __forceinline__ void write_loss(const List& list, const RowsParams& P, int64_t row, Stat st, bool none, bool bad) {
+  const float loss = list_loss(list, P.list.top, st, P.c, P.temperature);
   if ((threadIdx.x & 31) == 0) {
-    P.loss[row] = sh.none ? 0.f : sh.bad ? NAN : loss;
-    P.lse[row] = sh.none ? 0.f : sum_lse(st, P.c, P.temperature);
-    if (P.stats) P.stats[row] = make_float2(st.m, sh.none ? 0.f : st.s);
+    P.loss[row] = none ? 0.f : bad ? NAN : loss;
+    P.lse[row] = none ? 0.f : sum_lse(st, P.c, P.temperature);
+    if (P.stats) P.stats[row] = make_float2(st.m, none ? 0.f : st.s);
   }
 }
 
@@ -313,26 +316,61 @@ __global__ void __launch_bounds__(kSumThreads + 32, kSumCtas) distill_forward_ke
   if (tid >= S) {
     prepare_list<DT>(sh, P, row, 0, P.vocab);
   } else {
-    const Stat st = warp_merge(sum_span<DT, S, kSumStep>(span_of<DT>(P, P.z, P.ld, row, part), P.c, &sh.none, false), P.c);
+    const Stat st = warp_merge(sum_span<DT, S, kSumStep>(span_of<DT>(P, P.z, P.ld, row, part), tid, P.c, &sh.none, false), P.c);
     if ((tid & 31) == 0) sh.red[tid / 32] = st;
   }
   finish_sum<S>(sh, parts, P.c);
-  if (tid >= S && part == 0) write_loss<S>(sh, P, row, final_stat(sh.total, sh.bad));
+  if (tid >= S && part == 0)
+    write_loss(List(sh.list, kMaxTop), P, row, final_stat(sh.total, sh.bad), sh.none, sh.bad);
   leave(parts);
+}
+
+// Whether all indices of a list differ, by a hash table in the place of `order`, half full at most.
+__device__ __forceinline__ bool list_distinct(const List& s, int top) {
+  const int lane = threadIdx.x & 31, size = 2 * list_capacity(top);
+  int32_t* table = reinterpret_cast<int32_t*>(s.order);
+  for (int q = lane; q < size; q += 32) table[q] = -1;
+  __syncwarp();
+  bool twice = false;
+  for (int k = lane; k < top; k += 32) {
+    const int32_t own = s.idx[k];
+    if (own < 0) continue;
+    uint32_t at = (uint32_t)own * 2654435761u >> 16;   // Knuth's multiplicative hashing
+    for (;; ++at) {
+      const int32_t was = atomicCAS(table + (at & (size - 1)), -1, own);
+      if (was == -1) break;
+      if (was == own) {
+        twice = true;
+        break;
+      }
+    }
+  }
+  twice = __any_sync(0xffffffffu, twice);
+  __syncwarp();
+  return !twice;
 }
 
 // The gradient at the listed indices is A q - B (the sum of p over the entries with that
 // index): list_sums leaves that sum, in list order, in lp, and patch writes the gradient over
-// the dense part's value there. Entries that share an index write the same value.
-__device__ __forceinline__ void list_sums(List& s, int top) {
-  __syncwarp();
-  for (int k = threadIdx.x & 31; k < top; k += 32) {
-    const int32_t own = s.idx[k];
-    float a = 0.f;
-#pragma unroll 8
-    for (int j = 0; j < top; ++j) a += s.idx[j] == own ? s.p[j] : 0.f;
-    s.lp[k] = a;
+// the dense part's value there. Entries that share an index write the same value. Teachers' lists
+// seldom hold an index twice: only then are they sorted.
+__device__ __forceinline__ void list_sums(const List& s, int top) {
+  const int lane = threadIdx.x & 31;
+  if (list_distinct(s, top)) {
+    for (int k = lane; k < top; k += 32) s.lp[k] = s.p[k];
+    return;
   }
+  list_sort(s, top, [](int32_t idx) { return (uint32_t)idx; });
+  for (int q = lane; q < top; q += 32) {
+    const uint32_t own = (uint32_t)(s.order[q] >> 32);
+    if (own == 0xffffffffu) break;   // no mass from here on
+    int first = q;   // equal indices stand together, in list order
+    while (first > 0 && (uint32_t)(s.order[first - 1] >> 32) == own) --first;
+    float a = 0.f;
+    for (int r = first; r < top && (uint32_t)(s.order[r] >> 32) == own; ++r) a += s.p[(uint32_t)s.order[r]];
+    s.lp[(uint32_t)s.order[q]] = a;
+  }
+  __syncwarp();
 }
 
 template <int DT>
@@ -393,15 +431,16 @@ template <int DT> struct Dense {
 // for anything, and each step is loaded before the one before it is written. SAME: the gradient's
 // vectors are as aligned as the logits'.
 template <int DT, int S, int U, bool FOLD, bool SAME>
-__device__ __forceinline__ void write_vecs(uint4 (&u)[U], const Span<DT>& sp, typename El<DT>::T* out, const Dense<DT>& D, float c) {
+__device__ __forceinline__ void write_vecs(uint4 (&u)[U], const Span<DT>& sp, int tid, typename El<DT>::T* out, const Dense<DT>& D,
+                                           float c) {
   using T = typename El<DT>::T;
   constexpr int V = El<DT>::kVec;
   const int n = steps_of<DT, S, U>(sp);
-  int i = threadIdx.x;
+  int i = tid;
   T* o = out + sp.body + i * V;
   uint4 next[U];
   for (int g = 0; g < n; ++g) {
-    if (g + 1 < n) load_step<DT, S, U>(next, sp, g + 1, false);
+    if (g + 1 < n) load_step<DT, S, U>(next, sp, tid, g + 1, false);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const uint4 r = D.template vec<FOLD>(u[j], c);
@@ -423,20 +462,19 @@ __device__ __forceinline__ void write_vecs(uint4 (&u)[U], const Span<DT>& sp, ty
 
 // The stream threads' part of a row's gradient over a span. out has its own 16-byte phase.
 template <int DT, int S, int U>
-__device__ __forceinline__ void write_span(uint4 (&u)[U], const Span<DT>& sp, typename El<DT>::T* out, const Dense<DT>& D, float c) {
-  const int tid = threadIdx.x;
-  if (((uintptr_t)(out + sp.body) & 15) != 0) write_vecs<DT, S, U, false, false>(u, sp, out, D, c);
-  else if (DT != ZT_F32 && D.fold) write_vecs<DT, S, U, true, true>(u, sp, out, D, c);
-  else write_vecs<DT, S, U, false, true>(u, sp, out, D, c);
+__device__ __forceinline__ void write_span(uint4 (&u)[U], const Span<DT>& sp, int tid, typename El<DT>::T* out, const Dense<DT>& D,
+                                           float c) {
+  if (((uintptr_t)(out + sp.body) & 15) != 0) write_vecs<DT, S, U, false, false>(u, sp, tid, out, D, c);
+  else if (DT != ZT_F32 && D.fold) write_vecs<DT, S, U, true, true>(u, sp, tid, out, D, c);
+  else write_vecs<DT, S, U, false, true>(u, sp, tid, out, D, c);
   if (tid < sp.body - sp.lo) out[sp.lo + tid] = D.one(sp.row[sp.lo + tid], c);
   if (tid < sp.hi - sp.tail()) out[sp.tail() + tid] = D.one(sp.row[sp.tail() + tid], c);
 }
 
 // The gradient of a row without a teacher.
 template <int DT, int S>
-__device__ __forceinline__ void zero_span(typename El<DT>::T* out, int32_t lo, int32_t hi) {
+__device__ __forceinline__ void zero_span(typename El<DT>::T* out, int tid, int32_t lo, int32_t hi) {
   const Span<DT> o(out, lo, hi);
-  const int tid = threadIdx.x;
   const typename El<DT>::T zero = El<DT>::from(0.f);
   uint4* v = reinterpret_cast<uint4*>(out + o.body);
   for (int i = tid; i < o.n_vec; i += S) v[i] = make_uint4(0, 0, 0, 0);
@@ -448,7 +486,8 @@ template <int DT>
 __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backward_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
   constexpr int S = kWriteThreads, U = kWriteStep;
-  __shared__ List list;
+  __shared__ unsigned long long list_room[kMaxTop * List::kBytes / 8];
+  const List list(list_room, kMaxTop);
   // last rows first: those the forward read last may still be in L2
   const unsigned place = gridDim.x - 1 - blockIdx.x;
   const int64_t row = place / P.parts;
@@ -456,7 +495,7 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backwa
   const int tid = threadIdx.x;
   const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
   uint4 u[U];
-  if (tid < S) load_step<DT, S, U>(u, sp, 0, false);
+  if (tid < S) load_step<DT, S, U>(u, sp, tid, 0, false);
   const float2 s2 = P.stats[row];
   const Stat st{s2.x, s2.y};
   T* out = static_cast<T*>(P.grad) + row * P.ld_grad;
@@ -470,8 +509,8 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backwa
   }
   if (P.grad == P.z) __syncthreads();   // in place: the listed logits are read before they are overwritten
   if (tid < S) {
-    if (none) zero_span<DT, S>(out, sp.lo, sp.hi);
-    else write_span<DT, S, U>(u, sp, out, Dense<DT>(st, A, P.c), P.c);
+    if (none) zero_span<DT, S>(out, tid, sp.lo, sp.hi);
+    else write_span<DT, S, U>(u, sp, tid, out, Dense<DT>(st, A, P.c), P.c);
   }
   __syncthreads();
   if (tid >= S && !none) patch<DT>(list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
@@ -492,13 +531,14 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_grad_k
   const Span<DT> sp = span_of<DT>(P, P.z, P.ld, row, part);
   if (tid == 0) sh.none = 0;
   __syncthreads();
+  const List list(sh.list, kMaxTop);
   uint4 u[U];
   if (tid >= S) {
     prepare_list<DT>(sh, P, row, 0, P.vocab);   // in place: all of it before any part writes
   } else {
-    const Stat st = warp_merge(sum_span<DT, S, U>(sp, P.c, &sh.none, true), P.c);
+    const Stat st = warp_merge(sum_span<DT, S, U>(sp, tid, P.c, &sh.none, true), P.c);
     if ((tid & 31) == 0) sh.red[tid / 32] = st;
-    load_step<DT, S, U>(u, sp, 0, false);
+    load_step<DT, S, U>(u, sp, tid, 0, false);
   }
   finish_sum<S>(sh, parts, P.c);
   const bool none = sh.none;
@@ -506,16 +546,73 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_grad_k
   const float B = P.g[row] * P.temperature, A = B + (P.g_lse ? P.g_lse[row] / P.temperature : 0.f);
   T* out = static_cast<T*>(P.grad) + row * P.ld_grad;
   if (tid >= S) {
-    if (part == 0) write_loss<S>(sh, P, row, st);
-    list_sums(sh.list, P.list.top);   // after the loss: it takes the place of log2 p
+    if (part == 0) write_loss(list, P, row, st, none, sh.bad);
+    list_sums(list, P.list.top);   // after the loss: it takes the place of log2 p
   } else if (none) {
-    zero_span<DT, S>(out, sp.lo, sp.hi);
+    zero_span<DT, S>(out, tid, sp.lo, sp.hi);
   } else {
-    write_span<DT, S, U>(u, sp, out, Dense<DT>(st, A, P.c), P.c);
+    write_span<DT, S, U>(u, sp, tid, out, Dense<DT>(st, A, P.c), P.c);
   }
   __syncthreads();
-  if (tid >= S && !none) patch<DT>(sh.list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
+  if (tid >= S && !none) patch<DT>(list, P.list.top, st, A, B, P.c, out, sp.lo, sp.hi);
   leave(parts);
+}
+
+// Many short rows: a warp takes a row by itself, list and all. SUM: forward; WRITE: backward;
+// both: loss and gradient at once. (A CTA's start, its list and its end take about 5 us whatever
+// the row's length, and an SM has two to six CTAs under way, but 32 and more of these warps.)
+template <int DT, bool SUM, bool WRITE>
+__global__ void __launch_bounds__(32 * kRowWarps) distill_warp_kernel(const __grid_constant__ RowsParams P, int64_t rows, int cap) {
+  using T = typename El<DT>::T;
+  constexpr int U = 4;
+  extern __shared__ unsigned long long room[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + warp;
+  if (row >= rows) return;
+  const List list(room + (size_t)warp * cap * (List::kBytes / 8), cap);
+  const Span<DT> sp(static_cast<const T*>(P.z) + row * P.ld, 0, P.vocab);
+  T* out = WRITE ? static_cast<T*>(P.grad) + row * P.ld_grad : nullptr;
+  Stat st{0.f, 0.f};
+  bool none;
+  if (SUM) {
+    const Teacher t = read_list(list, P.list, row);
+    none = !t.any;
+    if (none) {
+      if (lane == 0) {
+        P.loss[row] = P.lse[row] = 0.f;
+        if (P.stats) P.stats[row] = make_float2(0.f, 0.f);
+      }
+    } else {
+      gather<DT>(list, sp.row, P.list.top, 0, P.vocab);
+      st = warp_merge(sum_span<DT, 32, U>(sp, lane, P.c, nullptr, WRITE), P.c);
+      st.m = __shfl_sync(0xffffffffu, st.m, 0);
+      st.s = __shfl_sync(0xffffffffu, st.s, 0);
+      st = final_stat(st, t.bad);
+      list_softmax(list, P.list.top, P.c);
+      write_loss(list, P, row, st, false, t.bad);
+    }
+  } else {
+    const float2 s2 = P.stats[row];
+    st = Stat{s2.x, s2.y};
+    none = st.s == 0.f;
+    if (!none) {
+      read_list(list, P.list, row);
+      gather<DT>(list, sp.row, P.list.top, 0, P.vocab);
+      list_softmax(list, P.list.top, P.c);
+    }
+  }
+  if (!WRITE) return;
+  if (none) {
+    zero_span<DT, 32>(out, lane, 0, P.vocab);
+    return;
+  }
+  uint4 u[U];
+  load_step<DT, 32, U>(u, sp, lane, 0, false);
+  const float B = (P.g ? P.g[row] : 0.f) * P.temperature, A = B + (P.g_lse ? P.g_lse[row] / P.temperature : 0.f);
+  list_sums(list, P.list.top);   // in place: its logits have been gathered
+  write_span<DT, 32, U>(u, sp, lane, out, Dense<DT>(st, A, P.c), P.c);
+  __syncwarp();
+  patch<DT>(list, P.list.top, st, A, B, P.c, out, 0, P.vocab);
 }
 
 int check_rows(const zt_distill_args* a, bool grad, const std::string& who) {
@@ -600,6 +697,30 @@ int launch(K kernel, int threads, const RowsParams& P, int64_t rows, bool cluste
   return zt::check_cuda(cudaLaunchKernelEx(&cfg, kernel, P), who);
 }
 
+// Whether a warp takes a row by itself: where the CTAs would need more waves than there are 8 KB in
+// a row (a wave of short rows takes about 5 us, a warp's row 4 us and 6 for each 8 KB), up to
+// 48 KB (2000 x 8000 bf16, loss and gradient: 24 us so, 65 a row to a CTA; 8000 x 32000: 340 and 325).
+constexpr int64_t kShortRow = 48 * 1024, kShortStep = 8 * 1024;
+
+bool short_rows(const zt_distill_args* a, int ctas) {
+  const int64_t bytes = row_bytes(a), slots = (int64_t)zt::sm_count() * ctas;
+  return bytes <= kShortRow && a->rows * kShortStep > slots * (bytes > kShortStep ? bytes : kShortStep);
+}
+
+template <int DT, bool SUM, bool WRITE>
+int launch_warps(const zt_distill_args* a, cudaStream_t s, const char* who) {
+  const int cap = list_capacity(a->top);
+  distill_warp_kernel<DT, SUM, WRITE><<<(unsigned)((a->rows + kRowWarps - 1) / kRowWarps), 32 * kRowWarps,
+                                       (size_t)kRowWarps * cap * List::kBytes, s>>>(rows_params(a, 1), a->rows, cap);
+  return zt::check_cuda(cudaGetLastError(), who);
+}
+
+template <bool SUM, bool WRITE> int launch_warps(const zt_distill_args* a, cudaStream_t s, const char* who) {
+  if (a->dtype == ZT_BF16) return launch_warps<ZT_BF16, SUM, WRITE>(a, s, who);
+  if (a->dtype == ZT_F16) return launch_warps<ZT_F16, SUM, WRITE>(a, s, who);
+  return launch_warps<ZT_F32, SUM, WRITE>(a, s, who);
+}
+
 }  // namespace
 
 extern "C" {
@@ -609,6 +730,7 @@ int zt_distill_rows(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, false, "zt_distill_rows")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->loss || !a->lse) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows: null pointer");
+  if (short_rows(a, kSumCtas)) return launch_warps<true, false>(a, zt::as_stream(stream), "zt_distill_rows launch");
   const RowsParams P = rows_params(a, parts_for(a, kSumCtas));
   auto* kernel = a->dtype == ZT_BF16 ? distill_forward_kernel<ZT_BF16>
                  : a->dtype == ZT_F16 ? distill_forward_kernel<ZT_F16> : distill_forward_kernel<ZT_F32>;
@@ -620,6 +742,7 @@ int zt_distill_rows_backward(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, true, "zt_distill_rows_backward")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->stats) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_backward: null pointer");
+  if (short_rows(a, kWriteCtas)) return launch_warps<false, true>(a, zt::as_stream(stream), "zt_distill_rows_backward launch");
   const RowsParams P = rows_params(a, parts_for(a, kWriteCtas));
   auto* kernel = a->dtype == ZT_BF16 ? distill_backward_kernel<ZT_BF16>
                  : a->dtype == ZT_F16 ? distill_backward_kernel<ZT_F16> : distill_backward_kernel<ZT_F32>;
@@ -631,6 +754,7 @@ int zt_distill_rows_grad(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, true, "zt_distill_rows_grad")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->loss || !a->lse || !a->weight) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_grad: null pointer");
+  if (short_rows(a, kWriteCtas)) return launch_warps<true, true>(a, zt::as_stream(stream), "zt_distill_rows_grad launch");
   const RowsParams P = rows_params(a, parts_for_grad(a));
   auto* kernel = a->dtype == ZT_BF16 ? distill_grad_kernel<ZT_BF16>
                  : a->dtype == ZT_F16 ? distill_grad_kernel<ZT_F16> : distill_grad_kernel<ZT_F32>;

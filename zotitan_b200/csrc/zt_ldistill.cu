@@ -16,10 +16,11 @@
 //    accumulator takes 1024 of K, and the epilogue threads add these up in registers, rounding
 //    to nearest: 0.9e-6 at any K, for 1.5% of the time (512 of K: 0.4e-6 for 6%).
 //    An epilogue thread owns half an accumulator row, 128 columns; two warps share 32 rows.
-//    The first of them also follows its rows' sorted lists through the tiles: a listed logit is
-//    fetched by a one-column load of tensor memory at that column (the column is the same
-//    for the warp's 32 rows, so a warp makes at most one such load per listed token of its
-//    rows and tile: about four at 64 entries of 128256 tokens), a part for each 1024 of K.
+//    Each also follows the part of its row's list that lies in its columns through the tiles: a
+//    listed logit is fetched by a one-column load of tensor memory at that column (the
+//    column is the same for the warp's 32 rows, so a warp makes at most one such load per
+//    listed token of its rows and half tile: about two at 64 entries of 128256 tokens), a
+//    part for each 1024 of K.
 // 3. combine_kernel: a row's sums over the splits, then its list's logits from their parts.
 // Every mbarrier wait is bounded; on expiry the kernel records an error
 // (zt_linear_distill_take_error), drains its own copies and MMAs and frees its tensor memory.
@@ -42,7 +43,11 @@ constexpr uint32_t kStageA = kHalfRows * kBK * 2;  // 16 KB of X
 constexpr uint32_t kStageBytes = 2 * kStageA;       // + 16 KB of W (this CTA's half of the N tile)
 constexpr int kTile = 256;
 constexpr uint32_t kTmemCols = 2 * kTile;
-constexpr size_t kSmem = 1024 + kStages * kStageBytes + 256;
+constexpr int kWindow = 16;    // entries of a row's list that an epilogue thread has at hand: two
+                               // halves, one in use and one on its way
+constexpr int kHalfShift = 24; // takes the bit of a column's half tile (128) to bit 31
+static_assert((kTile / 2) << kHalfShift == (int)0x80000000, "the half's bit leads the sorting key");
+constexpr size_t kSmem = 1024 + kStages * kStageBytes + 256 + kWindow * 32 * kEpilogueWarps * 4;
 constexpr uint32_t kIdesc = idesc_bf16(256, 256);
 constexpr int kListWarps = 8;
 enum { kHasTeacher = 0, kNoTeacher = 1, kBadIndex = 2 };
@@ -53,8 +58,9 @@ struct Params {
   CUtensorMap tmap_x;  // X [rows, k], box {64, 128}
   CUtensorMap tmap_w;  // W [vocab, k], box {64, 128}
   TopList list;
-  int32_t* status;     // [rows]
-  int32_t* idx;        // [rows][top] tokens in rising order, INT32_MAX behind the last with mass
+  int32_t* status;     // [rows]: 4 x (entries of the first half columns) + one of the above
+  int32_t* idx;        // [rows][top] tokens, those of the first half columns of their tiles, then those
+                       // of the second, each in rising order; INT32_MAX behind the last with mass
   float* lp;           // [rows][top] log2 p in that order
   float* z;            // [n_chunks][rows][top] logits in that order, a part for each chunk of K
   float2* partials;    // [2 n_splits][rows_pad] (m, s), of both halves of a split's tiles
@@ -71,29 +77,27 @@ __global__ void __launch_bounds__(32 * kListWarps) list_kernel(const __grid_cons
   const int64_t row = (int64_t)blockIdx.x * kListWarps + threadIdx.x / 32;
   if (row >= P.rows) return;
   const int lane = threadIdx.x & 31;
-  __shared__ List lists[kListWarps];
-  List& s = lists[threadIdx.x / 32];
+  __shared__ unsigned long long room[kListWarps][kMaxTop * List::kBytes / 8];
+  const List s(room[threadIdx.x / 32], kMaxTop);
   const Teacher t = read_list(s, P.list, row);
   list_softmax(s, P.top, P.c);
   for (int k = lane; k < P.top; k += 32)
-    if (s.p[k] == 0.f) s.idx[k] = INT32_MAX;   // no mass: behind the others
-  if (lane < (-P.top & 3)) s.idx[P.top + lane] = INT32_MAX;   // up to a whole 16 bytes
-  __syncwarp();
-  // an entry's place: those with a smaller token, or the same and an earlier place
-  for (int k = lane; k < P.top; k += 32) {
-    const int32_t own = s.idx[k];
-    int place = 0;
-#pragma unroll 4
-    for (int j = 0; j < P.top; j += 4) {   // behind the list stands INT32_MAX: never before an entry
-      const int4 o = *reinterpret_cast<const int4*>(s.idx + j);
-      place += (o.x < own || (o.x == own && j < k)) + (o.y < own || (o.y == own && j + 1 < k)) +
-               (o.z < own || (o.z == own && j + 2 < k)) + (o.w < own || (o.w == own && j + 3 < k));
+    if (s.p[k] == 0.f) s.idx[k] = -1;   // no mass: behind the others
+  // tokens of the first half of a tile's columns stand before those of the second, both rising
+  list_sort(s, P.top, [](int32_t idx) { return idx < 0 ? 0xffffffffu : (uint32_t)idx | ((uint32_t)idx & (kTile / 2)) << kHalfShift; });
+  int first = 0;
+  for (int k0 = 0; k0 < P.top; k0 += 32) {
+    const int k = k0 + lane;
+    uint32_t key = 0xffffffffu;
+    if (k < P.top) {
+      const unsigned long long e = s.order[k];
+      key = (uint32_t)(e >> 32);
+      P.idx[row * P.top + k] = key == 0xffffffffu ? INT32_MAX : (int32_t)(key & 0x7fffffffu);
+      P.lp[row * P.top + k] = s.lp[(uint32_t)e];
     }
-    const int64_t at = row * P.top + place;
-    P.idx[at] = own;
-    P.lp[at] = s.lp[k];
+    first += __popc(__ballot_sync(0xffffffffu, key < 0x80000000u));
   }
-  if (lane == 0) P.status[row] = !t.any ? kNoTeacher : t.bad ? kBadIndex : kHasTeacher;
+  if (lane == 0) P.status[row] = first << 2 | (!t.any ? kNoTeacher : t.bad ? kBadIndex : kHasTeacher);
 }
 
 __device__ __forceinline__ void item_range(const Params& P, int item, int& mt, int& split, int& nt0, int& nt1) {
@@ -133,6 +137,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* drain = bars + 2 * kStages + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int32_t* windows = reinterpret_cast<int32_t*>(smem + kStages * kStageBytes + 256);   // [kWindow][epilogue threads]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
@@ -243,25 +248,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int mt, split, nt0, nt1;
       item_range(P, item, mt, split, nt0, nt1);
       const int row = mt * kTile + (int)rank * (int)kHalfRows + row_local;
-      // the row's list from this split's first column on: its place, its next two tokens
+      // the row's entries of this half's columns, from this split's first column on
       const int32_t* list = P.idx + (int64_t)row * P.top;
-      int pos = P.top, next = INT32_MAX, after = INT32_MAX;
-      if (half == 0 && row < P.rows) {
-        int lo = 0, hi = nt0 > 0 ? P.top : 0;
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (list[mid] < nt0 * kTile) lo = mid + 1;
+      int pos = 0, end = 0, next = INT32_MAX;
+      int32_t* window = windows + (warp - 2) * 32 + lane;   // place p in slot p mod kWindow
+      auto fetch = [&](int from) {   // half a window's entries from `from` on
+#pragma unroll
+        for (int j = 0; j < kWindow / 2; ++j)
+          if (from + j < end)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                         ::"r"(smem_u32(window + ((from + j) & (kWindow - 1)) * 32 * kEpilogueWarps)), "l"(list + from + j)
+                         : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      auto arrived = [] { asm volatile("cp.async.wait_group 0;" ::: "memory"); };
+      auto look = [&]() { next = pos < end ? *(volatile int32_t*)(window + (pos & (kWindow - 1)) * 32 * kEpilogueWarps) : INT32_MAX; };
+      auto start = [&]() {   // at pos, with nothing at hand
+        arrived();
+        fetch(pos & ~(kWindow / 2 - 1));
+        fetch((pos & ~(kWindow / 2 - 1)) + kWindow / 2);
+        arrived();
+        look();
+      };
+      auto step = [&]() {   // to the next place
+        if ((++pos & (kWindow / 2 - 1)) == 0) {
+          arrived();
+          fetch(pos + kWindow / 2);
+        }
+        look();
+      };
+      if (row < P.rows) {
+        const int firsts = P.status[row] >> 2;
+        pos = half ? firsts : 0;
+        end = half ? P.top : firsts;
+        int hi = nt0 > 0 ? end : pos;
+        while (pos < hi) {
+          const int mid = (pos + hi) >> 1;
+          if (list[mid] < nt0 * kTile) pos = mid + 1;
           else hi = mid;
         }
-        pos = lo;
-        if (pos < P.top) next = list[pos];
-        if (pos + 1 < P.top) after = list[pos + 1];
+        start();
       }
+      __syncwarp();
       Stat st{-INFINITY, 0.f};
       for (int nt = nt0; ok && nt < nt1; ++nt) {
         const int tile0 = nt * kTile;
         float sum[kTile / 2];
-        const int pos0 = pos, next0 = next;
+        const int pos0 = pos;
         for (int ch = 0; ch < P.n_chunks; ++ch, ++tcount) {
           const uint32_t b = tcount & 1;
           int okw = 1;
@@ -283,32 +316,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               for (int j = 0; j < 16; ++j) sum[c0 + j] += __uint_as_float(r[j]);
             }
           }
-          if (half == 0) {
+          if (pos != pos0) {   // the tile's columns again, for this chunk
+            const bool gone = (pos ^ pos0) & ~(kWindow / 2 - 1);   // its half has been replaced
             pos = pos0;
-            next = next0;
-            bool fresh = true;
-            float* z = P.z + ((int64_t)ch * P.rows + row) * P.top;
-            for (;;) {  // the listed columns of this tile, one column of the warp's rows at a time
-              const int col = __reduce_min_sync(0xffffffffu, next);   // each column once, in order
-              if (col >= tile0 + kTile) break;
-              const float v = tmem_ld1(acc + (uint32_t)(col - tile0));
-              while (next == col) {   // again where the token stands in the list several times
-                z[pos] = v;
-                ++pos;
-                // `after` is loaded once a tile: a load here would hold up the whole warp at its
-                // next turn, and a row seldom has two tokens in a tile
-                next = fresh ? after : pos < P.top ? list[pos] : INT32_MAX;
-                fresh = false;
-              }
-              __syncwarp();
+            if (gone) start();
+            else look();
+          }
+          __syncwarp();
+          float* z = P.z + ((int64_t)ch * P.rows + row) * P.top;
+          for (;;) {  // the listed columns of this half, one column of the warp's rows at a time
+            const int col = __reduce_min_sync(0xffffffffu, next);   // each column once, in order
+            if (col >= tile0 + kTile) break;
+            const float v = tmem_ld1(acc + (uint32_t)(col - tile0));
+            while (next == col) {   // again where the token stands in the list several times
+              z[pos] = v;
+              step();
             }
+            __syncwarp();
           }
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(b ? leader_acce1 : leader_acce0);  // accumulator b may be overwritten
         }
         if (!ok) break;
-        if (pos != pos0) after = pos + 1 < P.top ? list[pos + 1] : INT32_MAX;
         const int col0 = tile0 + half * (kTile / 2);
         if (col0 + kTile / 2 > P.vocab) {  // the padded columns of the last tile
 #pragma unroll
@@ -317,6 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         absorb(st, sum, P.c);
       }
+      arrived();   // the windows serve the next item's rows
       if (ok && row < P.rows) P.partials[(size_t)(2 * split + half) * P.rows_pad + row] = make_float2(st.m, st.s);
     }
   }
@@ -359,7 +390,7 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
       z[e] = logit(at);   // not written where idx is INT32_MAX, and then not looked at
     }
   }
-  if (row < P.rows) status = __ldg(P.status + row);
+  if (row < P.rows) status = __ldg(P.status + row) & 3;
   Stat st{-INFINITY, 0.f};
 #pragma unroll 4
   for (int sp = tid / kCombineRows; sp < 2 * P.n_splits; sp += 32 * kListWarps / kCombineRows) {   // rows_pad covers the block
