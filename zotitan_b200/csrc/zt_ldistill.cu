@@ -15,13 +15,11 @@
 //    accumulate: over a K of 2048 that alone puts the loss 1.8e-6 off, over 4096 3.6e-6. So an
 //    accumulator takes 1024 of K, and the epilogue threads add these up in registers, rounding
 //    to nearest: 0.9e-6 at any K, for 1.5% of the time (512 of K: 0.4e-6 for 6%).
-//    An epilogue thread owns half an accumulator row, 128 columns; two warps share 32 rows.
-//    Each also follows the part of its row's list that lies in its columns through the tiles: a
-//    listed logit is fetched by a one-column load of tensor memory at that column (the
-//    column is the same for the warp's 32 rows, so a warp makes at most one such load per
-//    listed token of its rows and half tile: about two at 64 entries of 128256 tokens), a
-//    part for each 1024 of K.
-// 3. combine_kernel: a row's sums over the splits, then its list's logits from their parts.
+//    An epilogue thread owns half an accumulator row, 128 columns. It also follows the part of
+//    its row's list that lies in its columns through the tiles: where one of a warp's rows has
+//    a listed token among 16 columns, its threads put theirs into shared memory, each for itself,
+//    and pick theirs out by index.
+// 3. combine_kernel: a row's sums over the splits, then its list.
 // Every mbarrier wait is bounded; on expiry the kernel records an error
 // (zt_linear_distill_take_error), drains its own copies and MMAs and frees its tensor memory.
 #include <math.h>
@@ -43,11 +41,12 @@ constexpr uint32_t kStageA = kHalfRows * kBK * 2;  // 16 KB of X
 constexpr uint32_t kStageBytes = 2 * kStageA;       // + 16 KB of W (this CTA's half of the N tile)
 constexpr int kTile = 256;
 constexpr uint32_t kTmemCols = 2 * kTile;
-constexpr int kWindow = 16;    // entries of a row's list that an epilogue thread has at hand: two
-                               // halves, one in use and one on its way
+constexpr int kWindow = 16;    // entries of a row's list that an epilogue thread has at hand
+constexpr int kSlab = 16;      // columns that it puts into shared memory to pick from
+constexpr int kLanes = 32 * kEpilogueWarps;
 constexpr int kHalfShift = 24; // takes the bit of a column's half tile (128) to bit 31
 static_assert((kTile / 2) << kHalfShift == (int)0x80000000, "the half's bit leads the sorting key");
-constexpr size_t kSmem = 1024 + kStages * kStageBytes + 256 + kWindow * 32 * kEpilogueWarps * 4;
+constexpr size_t kSmem = 1024 + kStages * kStageBytes + 256 + (kWindow + kSlab) * 32 * kEpilogueWarps * 4;
 constexpr uint32_t kIdesc = idesc_bf16(256, 256);
 constexpr int kListWarps = 8;
 enum { kHasTeacher = 0, kNoTeacher = 1, kBadIndex = 2 };
@@ -62,7 +61,7 @@ struct Params {
   int32_t* idx;        // [rows][top] tokens, those of the first half columns of their tiles, then those
                        // of the second, each in rising order; INT32_MAX behind the last with mass
   float* lp;           // [rows][top] log2 p in that order
-  float* z;            // [n_chunks][rows][top] logits in that order, a part for each chunk of K
+  float* z;            // [rows][top] logits in that order
   float2* partials;    // [2 n_splits][rows_pad] (m, s), of both halves of a split's tiles
   float* loss;
   float* lse;
@@ -115,13 +114,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
-  uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  return __uint_as_float(r);
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -250,32 +242,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int row = mt * kTile + (int)rank * (int)kHalfRows + row_local;
       // the row's entries of this half's columns, from this split's first column on
       const int32_t* list = P.idx + (int64_t)row * P.top;
+      float* z = P.z + (int64_t)row * P.top;
       int pos = 0, end = 0, next = INT32_MAX;
+      int have = 0, ready = 0;   // places before `have` have been fetched, before `ready` are at hand
       int32_t* window = windows + (warp - 2) * 32 + lane;   // place p in slot p mod kWindow
-      auto fetch = [&](int from) {   // half a window's entries from `from` on
+      float* slab = reinterpret_cast<float*>(window + kWindow * kLanes);
+      auto fetch = [&]() {   // the next half window
 #pragma unroll
         for (int j = 0; j < kWindow / 2; ++j)
-          if (from + j < end)
+          if (have + j < end)
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
-                         ::"r"(smem_u32(window + ((from + j) & (kWindow - 1)) * 32 * kEpilogueWarps)), "l"(list + from + j)
+                         ::"r"(smem_u32(window + ((have + j) & (kWindow - 1)) * kLanes)), "l"(list + have + j)
                          : "memory");
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        have += kWindow / 2;
       };
-      auto arrived = [] { asm volatile("cp.async.wait_group 0;" ::: "memory"); };
-      auto look = [&]() { next = pos < end ? *(volatile int32_t*)(window + (pos & (kWindow - 1)) * 32 * kEpilogueWarps) : INT32_MAX; };
-      auto start = [&]() {   // at pos, with nothing at hand
-        arrived();
-        fetch(pos & ~(kWindow / 2 - 1));
-        fetch((pos & ~(kWindow / 2 - 1)) + kWindow / 2);
-        arrived();
-        look();
+      auto arrived = [&]() {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        ready = have;
       };
-      auto step = [&]() {   // to the next place
-        if ((++pos & (kWindow / 2 - 1)) == 0) {
-          arrived();
-          fetch(pos + kWindow / 2);
+      auto look = [&]() {   // next <- the token at pos
+        if (pos >= end) {
+          next = INT32_MAX;
+          return;
         }
-        look();
+        while (pos >= ready) {   // only after more than half a window in one tile
+          if (pos >= have) fetch();
+          arrived();
+        }
+        next = *(volatile int32_t*)(window + (pos & (kWindow - 1)) * kLanes);
       };
       if (row < P.rows) {
         const int firsts = P.status[row] >> 2;
@@ -287,14 +281,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (list[mid] < nt0 * kTile) pos = mid + 1;
           else hi = mid;
         }
-        start();
+        arrived();   // what the last item's row had asked for
+        have = ready = pos;
+        fetch();
+        fetch();
+        look();
       }
       __syncwarp();
       Stat st{-INFINITY, 0.f};
       for (int nt = nt0; ok && nt < nt1; ++nt) {
         const int tile0 = nt * kTile;
         float sum[kTile / 2];
-        const int pos0 = pos;
+        arrived();   // asked for at the last tile
+        if (have - pos <= kWindow / 2 && have < end) fetch();
         for (int ch = 0; ch < P.n_chunks; ++ch, ++tcount) {
           const uint32_t b = tcount & 1;
           int okw = 1;
@@ -316,24 +315,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               for (int j = 0; j < 16; ++j) sum[c0 + j] += __uint_as_float(r[j]);
             }
           }
-          if (pos != pos0) {   // the tile's columns again, for this chunk
-            const bool gone = (pos ^ pos0) & ~(kWindow / 2 - 1);   // its half has been replaced
-            pos = pos0;
-            if (gone) start();
-            else look();
-          }
-          __syncwarp();
-          float* z = P.z + ((int64_t)ch * P.rows + row) * P.top;
-          for (;;) {  // the listed columns of this half, one column of the warp's rows at a time
-            const int col = __reduce_min_sync(0xffffffffu, next);   // each column once, in order
-            if (col >= tile0 + kTile) break;
-            const float v = tmem_ld1(acc + (uint32_t)(col - tile0));
-            while (next == col) {   // again where the token stands in the list several times
-              z[pos] = v;
-              step();
-            }
-            __syncwarp();
-          }
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(b ? leader_acce1 : leader_acce0);  // accumulator b may be overwritten
@@ -346,10 +327,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (col0 + j >= P.vocab) sum[j] = -INFINITY;
         }
         absorb(st, sum, P.c);
+#pragma unroll
+        for (int c0 = 0; c0 < kTile / 2; c0 += kSlab) {
+          if (!__any_sync(0xffffffffu, next < col0 + c0 + kSlab)) continue;
+#pragma unroll
+          for (int j = 0; j < kSlab; ++j) slab[j * kLanes] = sum[c0 + j];
+          while (next < col0 + c0 + kSlab) {   // once more where the token stands in the list several times
+            z[pos] = slab[(next - (col0 + c0)) * kLanes];
+            ++pos;
+            look();
+          }
+          __syncwarp();
+        }
       }
-      arrived();   // the windows serve the next item's rows
       if (ok && row < P.rows) P.partials[(size_t)(2 * split + half) * P.rows_pad + row] = make_float2(st.m, st.s);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");   // no copy is in flight when the thread leaves
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncwarp();
@@ -371,13 +364,6 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
   const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
   const int64_t row = row0 + warp;
   constexpr int kHeld = 4;   // list entries of a lane loaded ahead
-  const int64_t part_stride = (int64_t)P.rows * P.top;
-  auto logit = [&](int64_t at) {   // the parts in order
-    float v = 0.f;
-#pragma unroll 4
-    for (int ch = 0; ch < P.n_chunks; ++ch) v += __ldg(P.z + ch * part_stride + at);
-    return v;
-  };
   int32_t idx[kHeld], status = kNoTeacher;
   float lp[kHeld], z[kHeld];
 #pragma unroll
@@ -387,7 +373,7 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
       const int64_t at = row * P.top + lane + 32 * e;
       idx[e] = __ldg(P.idx + at);
       lp[e] = __ldg(P.lp + at);
-      z[e] = logit(at);   // not written where idx is INT32_MAX, and then not looked at
+      z[e] = __ldg(P.z + at);   // not written where idx is INT32_MAX, and then not looked at
     }
   }
   if (row < P.rows) status = __ldg(P.status + row) & 3;
@@ -420,7 +406,7 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
     if (idx[e] != INT32_MAX) add(lp[e], z[e]);
   for (int k = lane + 32 * kHeld; k < P.top; k += 32) {
     const int64_t at = row * P.top + k;
-    if (P.idx[at] != INT32_MAX) add(P.lp[at], logit(at));
+    if (P.idx[at] != INT32_MAX) add(P.lp[at], P.z[at]);
   }
   a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
   if (lane == 0) {
@@ -508,15 +494,13 @@ struct Layout {
   size_t idx, lp, z, status, total;
 };
 
-int32_t chunks_of(int64_t k) { return (int32_t)((k / kBK + kChunk - 1) / kChunk); }
-
-Layout layout(const Split& sp, int64_t rows, int32_t top, int32_t n_chunks) {
+Layout layout(const Split& sp, int64_t rows, int32_t top) {
   const size_t entries = (size_t)rows * (size_t)top * 4;
   Layout L;
   L.idx = up256(2 * sizeof(float2) * (size_t)sp.n_splits * (size_t)sp.rows_pad);
   L.lp = L.idx + up256(entries);
   L.z = L.lp + up256(entries);
-  L.status = L.z + up256(entries * (size_t)n_chunks);
+  L.status = L.z + up256(entries);
   L.total = L.status + up256((size_t)rows * 4);
   return L;
 }
@@ -530,7 +514,7 @@ size_t zt_linear_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k,
   if (check_shape(rows, vocab, k, top)) return 0;
   int dev = 0, pairs = 0;
   if (device_pairs(&dev, &pairs)) return 0;
-  return layout(choose_split(rows, vocab, pairs), rows, top, chunks_of(k)).total;
+  return layout(choose_split(rows, vocab, pairs), rows, top).total;
 }
 
 int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
@@ -547,7 +531,7 @@ int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
   int dev = 0, pairs = 0;
   if (int rc = device_pairs(&dev, &pairs)) return rc;
   const Split sp = choose_split(a->rows, a->vocab, pairs);
-  const Layout L = layout(sp, a->rows, a->top, chunks_of(a->k));
+  const Layout L = layout(sp, a->rows, a->top);
   if (a->workspace_bytes < L.total) return zt::set_error(ZT_ERR_INVALID, "zt_linear_distill: workspace too small");
   EncodeFn enc = nullptr;
   if (int rc = get_encode(&enc, "zt_linear_distill")) return rc;
@@ -569,7 +553,7 @@ int zt_linear_distill(const zt_linear_distill_args* a, void* stream) {
   P.vocab = (int32_t)a->vocab;
   P.top = a->top;
   P.k_blocks = (int32_t)(a->k / kBK);
-  P.n_chunks = chunks_of(a->k);
+  P.n_chunks = (P.k_blocks + kChunk - 1) / kChunk;
   P.m_tiles = sp.m_tiles;
   P.n_tiles = sp.n_tiles;
   P.split_tiles = sp.split_tiles;
