@@ -190,13 +190,14 @@ __device__ __forceinline__ int first_of(int before, int part, int split) {
 
 // ---- the plain kernels: single elements -------------------------------------------------------
 //
-// One warp a position and part of its heads. Weight, cos and sin enter as their products
+// One warp a position and part of its heads, NC elements of each half a lane (two up to heads of
+// 128, where eight would leave a quarter of the warps). Weight, cos and sin enter as their products
 // (w cos and w' sin, once per position), and n at the end:
 //   out[i] = n (x[i] (w[i] cos[i]) - x[i + h] (w[i + h] sin[i])), out[i + h] alike.
-template <int DT>
+template <int DT, int NC>
 __global__ void __launch_bounds__(32 * kWarps) qk_forward_kernel(const __grid_constant__ QkParams P) {
   using T = typename El<DT>::T;
-  constexpr int V = 1, NC = kE;
+  constexpr int V = 1;
   const int64_t item = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
   if (item >= (int64_t)P.rows * P.split) return;
   const int row = (int)(item / P.split), part = (int)(item - (int64_t)row * P.split);
@@ -294,10 +295,10 @@ __device__ __forceinline__ void block_weights(const QkParams& P, float (&dl)[2][
 
 // Persistent warps over (position, part of its heads); each lane sums its elements of the
 // weight gradients in registers, a block adds its warps' sums in warp order.
-template <int DT>
+template <int DT, int NC>
 __global__ void __launch_bounds__(32 * kBwdWarps) qk_backward_kernel(const __grid_constant__ QkParams P) {
   using T = typename El<DT>::T;
-  constexpr int V = 1, NC = kE;
+  constexpr int V = 1;
   extern __shared__ float sums[];   // [kBwdWarps][2][hd]
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int lanes = P.lanes, per_warp = 32 / lanes, sub = lane & (lanes - 1), mine = lane / lanes;
@@ -871,6 +872,13 @@ template <int DT, int LANES> int launch_ring(const QkParams& P, bool backward, i
   return ZT_OK;
 }
 
+template <int DT, int NC> void launch_plain(const QkParams& P, bool backward, int blocks, cudaStream_t s) {
+  if (backward)
+    qk_backward_kernel<DT, NC><<<blocks, 32 * kBwdWarps, sizeof(float) * kBwdWarps * 2 * P.hd, s>>>(P);
+  else
+    qk_forward_kernel<DT, NC><<<blocks, 32 * kWarps, 0, s>>>(P);
+}
+
 template <int DT> int launch_typed(const QkParams& P, bool backward, bool ring, int blocks, cudaStream_t s) {
   if (ring) {
     if (P.lanes == 4) return launch_ring<DT, 4>(P, backward, blocks, s);
@@ -878,10 +886,7 @@ template <int DT> int launch_typed(const QkParams& P, bool backward, bool ring, 
     if (P.lanes == 16) return launch_ring<DT, 16>(P, backward, blocks, s);
     return launch_ring<DT, 0>(P, backward, blocks, s);
   }
-  if (backward)
-    qk_backward_kernel<DT><<<blocks, 32 * kBwdWarps, sizeof(float) * kBwdWarps * 2 * P.hd, s>>>(P);
-  else
-    qk_forward_kernel<DT><<<blocks, 32 * kWarps, 0, s>>>(P);
+  P.half <= 64 ? launch_plain<DT, 2>(P, backward, blocks, s) : launch_plain<DT, kE>(P, backward, blocks, s);
   return ZT_OK;
 }
 
