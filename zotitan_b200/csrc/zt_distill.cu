@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backwa
 
 // Loss and gradient at once: the sum reads the row from memory, the gradient reads it again from
 // L2. (Held in the shared memory of a cluster of four instead, the row's loads, sums and
-// stores took turns, and 2048 x 128256 bf16 measured 256 us against 227.)
+// stores took turns: 2048 x 128256 bf16 257 us, so 213.)
 template <int DT>
 __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_grad_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
@@ -636,7 +636,7 @@ int check_rows(const zt_distill_args* a, bool grad, const std::string& who) {
 
 // CTAs of a row: doubled up to 8 while all of them still run at once, and a part keeps at least
 // kMinPart elements. (Splitting rows that fill the GPU's slots already, to even out their last
-// wave, costs more than it gives: 1001 x 50257 fp16 forward 34 us in two parts, 28 in one.)
+// wave, costs more than it gives: 1001 x 50257 fp16 forward 34 us in two parts, 27 in one.)
 constexpr int64_t kMinPart = 2048;
 
 int parts_for(const zt_distill_args* a, int ctas) {
@@ -649,9 +649,9 @@ int parts_for(const zt_distill_args* a, int ctas) {
 int64_t row_bytes(const zt_distill_args* a) { return a->vocab * (a->dtype == ZT_F32 ? 4 : 2); }
 
 // The same for loss and gradient at once, whose rows under way have to stay in L2 between their
-// two readings: at most kInFlight bytes of them (of 2048 x 128256 bf16, 76 MB under way
-// measured 227 us, 151 MB 254).
-constexpr int64_t kInFlight = 80ll << 20;
+// two readings: at most kInFlight bytes of them (2048 x 128256 fp32, 152 MB under way 450 us, in
+// two parts 424; 1500 x 200000 bf16, 118 MB: 263, in two parts 278).
+constexpr int64_t kInFlight = 128ll << 20;
 
 int parts_for_grad(const zt_distill_args* a) {
   const int64_t slots = (int64_t)zt::sm_count() * kWriteCtas;
@@ -699,7 +699,7 @@ int launch(K kernel, int threads, const RowsParams& P, int64_t rows, bool cluste
 
 // Whether a warp takes a row by itself: where the CTAs would need more waves than there are 8 KB in
 // a row (a wave of short rows takes about 5 us, a warp's row 4 us and 6 for each 8 KB), up to
-// 48 KB (2000 x 8000 bf16, loss and gradient: 24 us so, 65 a row to a CTA; 8000 x 32000: 340 and 325).
+// 48 KB (2000 x 8000 bf16, loss and gradient: 22 us so, 65 a row to a CTA; 8000 x 32000: 340 and 325).
 constexpr int64_t kShortRow = 48 * 1024, kShortStep = 8 * 1024;
 
 bool short_rows(const zt_distill_args* a, int ctas) {
