@@ -28,7 +28,12 @@ using zt::tc::peer_addr;
 // takes 180 us with six CTAs of two vectors, 184 with four of four, 199 to 226 where
 // a thread also loads its next step ahead (its registers cost warps).
 constexpr int kSumThreads = 256, kSumCtas = 6, kSumStep = 2;
-constexpr int kWriteThreads = 512, kWriteCtas = 2, kWriteStep = 4;   // backward, and loss and gradient at once
+// The backward, and loss and gradient at once: rows of up to kMidRow bytes go to CTAs half as wide,
+// twice as many (4000 x 32000 bf16, 64 KB: 117 us so, 152 with the wide ones; 2048 x 100000, 200 KB:
+// 189 and 179).
+constexpr int kWriteStep = 4;
+constexpr int kWideThreads = 512, kWideCtas = 2, kMidThreads = 256, kMidCtas = 4;
+constexpr int64_t kMidRow = 112 * 1024;
 constexpr int kRowWarps = 8;         // rows of a block where a warp takes a row
 constexpr int kMaxCluster = 8;
 
@@ -482,10 +487,10 @@ __device__ __forceinline__ void zero_span(typename El<DT>::T* out, int tid, int3
   if (tid < o.hi - o.tail()) out[o.tail() + tid] = zero;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backward_kernel(const __grid_constant__ RowsParams P) {
+template <int DT, int S, int CTAS>
+__global__ void __launch_bounds__(S + 32, CTAS) distill_backward_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
-  constexpr int S = kWriteThreads, U = kWriteStep;
+  constexpr int U = kWriteStep;
   __shared__ unsigned long long list_room[kMaxTop * List::kBytes / 8];
   const List list(list_room, kMaxTop);
   // last rows first: those the forward read last may still be in L2
@@ -519,10 +524,10 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_backwa
 // Loss and gradient at once: the sum reads the row from memory, the gradient reads it again from
 // L2. (Held in the shared memory of a cluster of four instead, the row's loads, sums and
 // stores took turns: 2048 x 128256 bf16 257 us, so 213.)
-template <int DT>
-__global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_grad_kernel(const __grid_constant__ RowsParams P) {
+template <int DT, int S, int CTAS>
+__global__ void __launch_bounds__(S + 32, CTAS) distill_grad_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;
-  constexpr int S = kWriteThreads, U = kWriteStep;
+  constexpr int U = kWriteStep;
   __shared__ Shared<S> sh;
   const int parts = P.parts;
   const int64_t row = blockIdx.x / parts;
@@ -560,7 +565,7 @@ __global__ void __launch_bounds__(kWriteThreads + 32, kWriteCtas) distill_grad_k
 
 // Many short rows: a warp takes a row by itself, list and all. SUM: forward; WRITE: backward;
 // both: loss and gradient at once. (A CTA's start, its list and its end take about 5 us whatever
-// the row's length, and an SM has two to six CTAs under way, but 32 and more of these warps.)
+// the row's length, and an SM has two to six CTAs under way, but 16 to 32 of these warps.)
 template <int DT, bool SUM, bool WRITE>
 __global__ void __launch_bounds__(32 * kRowWarps) distill_warp_kernel(const __grid_constant__ RowsParams P, int64_t rows, int cap) {
   using T = typename El<DT>::T;
@@ -653,9 +658,9 @@ int64_t row_bytes(const zt_distill_args* a) { return a->vocab * (a->dtype == ZT_
 // two parts 424; 1500 x 200000 bf16, 118 MB: 263, in two parts 278).
 constexpr int64_t kInFlight = 128ll << 20;
 
-int parts_for_grad(const zt_distill_args* a) {
-  const int64_t slots = (int64_t)zt::sm_count() * kWriteCtas;
-  int parts = parts_for(a, kWriteCtas);
+int parts_for_grad(const zt_distill_args* a, int ctas) {
+  const int64_t slots = (int64_t)zt::sm_count() * ctas;
+  int parts = parts_for(a, ctas);
   while (parts < kMaxCluster && slots / parts * row_bytes(a) > kInFlight && a->rows * parts >= slots) parts *= 2;
   return parts;
 }
@@ -697,14 +702,16 @@ int launch(K kernel, int threads, const RowsParams& P, int64_t rows, bool cluste
   return zt::check_cuda(cudaLaunchKernelEx(&cfg, kernel, P), who);
 }
 
-// Whether a warp takes a row by itself: where the CTAs would need more waves than there are 8 KB in
-// a row (a wave of short rows takes about 5 us, a warp's row 4 us and 6 for each 8 KB), up to
-// 48 KB (2000 x 8000 bf16, loss and gradient: 22 us so, 65 a row to a CTA; 8000 x 32000: 340 and 325).
-constexpr int64_t kShortRow = 48 * 1024, kShortStep = 8 * 1024;
+// Whether a warp takes a row by itself: rows of at most `most` bytes, where the CTAs would need more
+// waves than there are 8 KB in a row (a wave of short rows takes about 5 us, a warp's row 4 us
+// and 6 for each 8 KB). Measured on 64 entries of bf16, a warp against a CTA a row: forward
+// 8000 x 20000 74 and 84 us; backward 2000 x 8000 21.2 and 21.6, 2000 x 12000 28 and 25; loss and
+// gradient 8000 x 12000 122 and 147, 4000 x 16000 82 and 77.
+constexpr int64_t kShortSum = 48 * 1024, kShortWrite = 16 * 1024, kShortGrad = 24 * 1024, kShortStep = 8 * 1024;
 
-bool short_rows(const zt_distill_args* a, int ctas) {
+bool short_rows(const zt_distill_args* a, int64_t most, int ctas) {
   const int64_t bytes = row_bytes(a), slots = (int64_t)zt::sm_count() * ctas;
-  return bytes <= kShortRow && a->rows * kShortStep > slots * (bytes > kShortStep ? bytes : kShortStep);
+  return bytes <= most && a->rows * kShortStep > slots * (bytes > kShortStep ? bytes : kShortStep);
 }
 
 template <int DT, bool SUM, bool WRITE>
@@ -721,6 +728,24 @@ template <bool SUM, bool WRITE> int launch_warps(const zt_distill_args* a, cudaS
   return launch_warps<ZT_F32, SUM, WRITE>(a, s, who);
 }
 
+template <int DT> int launch_backward(const zt_distill_args* a, cudaStream_t s) {
+  const char* who = "zt_distill_rows_backward launch";
+  if (row_bytes(a) <= kMidRow)
+    return launch(distill_backward_kernel<DT, kMidThreads, kMidCtas>, kMidThreads + 32,
+                  rows_params(a, parts_for(a, kMidCtas)), a->rows, false, s, who);
+  return launch(distill_backward_kernel<DT, kWideThreads, kWideCtas>, kWideThreads + 32,
+                rows_params(a, parts_for(a, kWideCtas)), a->rows, false, s, who);
+}
+
+template <int DT> int launch_grad(const zt_distill_args* a, cudaStream_t s) {
+  const char* who = "zt_distill_rows_grad launch";
+  if (row_bytes(a) <= kMidRow)
+    return launch(distill_grad_kernel<DT, kMidThreads, kMidCtas>, kMidThreads + 32,
+                  rows_params(a, parts_for_grad(a, kMidCtas)), a->rows, true, s, who);
+  return launch(distill_grad_kernel<DT, kWideThreads, kWideCtas>, kWideThreads + 32,
+                rows_params(a, parts_for_grad(a, kWideCtas)), a->rows, true, s, who);
+}
+
 }  // namespace
 
 extern "C" {
@@ -730,7 +755,7 @@ int zt_distill_rows(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, false, "zt_distill_rows")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->loss || !a->lse) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows: null pointer");
-  if (short_rows(a, kSumCtas)) return launch_warps<true, false>(a, zt::as_stream(stream), "zt_distill_rows launch");
+  if (short_rows(a, kShortSum, kSumCtas)) return launch_warps<true, false>(a, zt::as_stream(stream), "zt_distill_rows launch");
   const RowsParams P = rows_params(a, parts_for(a, kSumCtas));
   auto* kernel = a->dtype == ZT_BF16 ? distill_forward_kernel<ZT_BF16>
                  : a->dtype == ZT_F16 ? distill_forward_kernel<ZT_F16> : distill_forward_kernel<ZT_F32>;
@@ -742,11 +767,11 @@ int zt_distill_rows_backward(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, true, "zt_distill_rows_backward")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->stats) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_backward: null pointer");
-  if (short_rows(a, kWriteCtas)) return launch_warps<false, true>(a, zt::as_stream(stream), "zt_distill_rows_backward launch");
-  const RowsParams P = rows_params(a, parts_for(a, kWriteCtas));
-  auto* kernel = a->dtype == ZT_BF16 ? distill_backward_kernel<ZT_BF16>
-                 : a->dtype == ZT_F16 ? distill_backward_kernel<ZT_F16> : distill_backward_kernel<ZT_F32>;
-  return launch(kernel, kWriteThreads + 32, P, a->rows, false, zt::as_stream(stream), "zt_distill_rows_backward launch");
+  cudaStream_t s = zt::as_stream(stream);
+  if (short_rows(a, kShortWrite, kMidCtas)) return launch_warps<false, true>(a, s, "zt_distill_rows_backward launch");
+  if (a->dtype == ZT_BF16) return launch_backward<ZT_BF16>(a, s);
+  if (a->dtype == ZT_F16) return launch_backward<ZT_F16>(a, s);
+  return launch_backward<ZT_F32>(a, s);
 }
 
 int zt_distill_rows_grad(const zt_distill_args* a, void* stream) {
@@ -754,11 +779,11 @@ int zt_distill_rows_grad(const zt_distill_args* a, void* stream) {
   if (int rc = check_rows(a, true, "zt_distill_rows_grad")) return rc;
   if (a->rows == 0) return ZT_OK;
   if (!a->loss || !a->lse || !a->weight) return zt::set_error(ZT_ERR_INVALID, "zt_distill_rows_grad: null pointer");
-  if (short_rows(a, kWriteCtas)) return launch_warps<true, true>(a, zt::as_stream(stream), "zt_distill_rows_grad launch");
-  const RowsParams P = rows_params(a, parts_for_grad(a));
-  auto* kernel = a->dtype == ZT_BF16 ? distill_grad_kernel<ZT_BF16>
-                 : a->dtype == ZT_F16 ? distill_grad_kernel<ZT_F16> : distill_grad_kernel<ZT_F32>;
-  return launch(kernel, kWriteThreads + 32, P, a->rows, true, zt::as_stream(stream), "zt_distill_rows_grad launch");
+  cudaStream_t s = zt::as_stream(stream);
+  if (short_rows(a, kShortGrad, kMidCtas)) return launch_warps<true, true>(a, s, "zt_distill_rows_grad launch");
+  if (a->dtype == ZT_BF16) return launch_grad<ZT_BF16>(a, s);
+  if (a->dtype == ZT_F16) return launch_grad<ZT_F16>(a, s);
+  return launch_grad<ZT_F32>(a, s);
 }
 
 }  // extern "C"
