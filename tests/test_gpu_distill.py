@@ -121,6 +121,13 @@ CASES = [
     (2, 70001, 100, "f32", 1.0, 70010, 1, torch.int64, torch.float32),
     (9, 2047, 7, "f16", 1.0, None, 1, torch.int64, torch.float32),
     (40, 151936, 16, "bf16", 1.0, None, 0, torch.int64, torch.float32),
+    # many short rows, a warp each
+    (1200, 1003, 33, "bf16", 2.0, 1008, 0, torch.int32, torch.bfloat16),
+    (1300, 777, 65, "f16", 1.0, None, 3, torch.int64, torch.float32),
+    (1000, 1501, 256, "f32", 0.7, 1510, 1, torch.int64, torch.float32),
+    (5000, 9, 4, "bf16", 1.0, None, 0, torch.int64, torch.float32),
+    # long rows, a wide CTA each
+    (310, 70001, 16, "f32", 1.0, None, 0, torch.int64, torch.float32),
 ]
 IDS = ["-".join(str(v) for v in c).replace("torch.", "") for c in CASES]
 
@@ -200,25 +207,32 @@ def test_rows_backward_against_differences():
         assert abs(float(terms.sum()) - want) <= 1e-5 * float(terms.abs().sum())
 
 
-def test_repeated_index():
+COPIES = pytest.mark.parametrize("copies", [1, 200])   # a CTA a row, and a warp a row
+
+
+@COPIES
+def test_repeated_index(copies):
     """The same token several times in a list: its masses add, in the loss and the gradient."""
     from zotitan_b200 import kernels as K
     z, idx, val = make(6, 1000, 70, torch.float32, seed=4, empty=False)
     idx[:, 40:] = idx[:, :30]
     idx[3] = 17
+    idx[4, 1::2] = -1
+    z, idx, val = (t.repeat(copies, 1) for t in (z, idx, val))
     e = Exact(z, idx, val, 1.0)
     leaf = z.detach().requires_grad_()
     loss, _ = K.distill_rows(leaf, idx, val)
     close(loss.detach(), e.loss, e.tol_loss, torch.float32)
-    g = torch.rand(6, device="cuda") + 0.5
+    g = torch.rand(6 * copies, device="cuda") + 0.5
     want, tol = e.grad(g)
     got, = torch.autograd.grad(loss, leaf, g)
     close(got, want, tol, torch.float32)
     close(K.distill_rows_grad(z, idx, val, g)[2], want, tol, torch.float32)
 
 
+@COPIES
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
-def test_masked_logits(dt):
+def test_masked_logits(dt, copies):
     """Student logits masked by -inf or the type's lowest value, teacher values likewise."""
     from zotitan_b200 import kernels as K
     dtype = DTYPES[dt]
@@ -230,36 +244,40 @@ def test_masked_logits(dt):
     z[2] = low                                        # nothing but the lowest: uniform
     val[3, 5:] = torch.finfo(torch.float32).min       # masked by value, mass underflows to 0
     val[4] = torch.finfo(torch.float32).min           # all alike: uniform
+    z, idx, val = (t.repeat(copies, 1) for t in (z, idx, val))
     e = Exact(z, idx, val, 1.0)
-    e.tol_lse[2] = U * 8 * abs(low)
+    e.tol_lse[2::8] = U * 8 * abs(low)
     leaf = z.detach().requires_grad_()
     loss, lse = K.distill_rows(leaf, idx, val)
     close(loss.detach(), e.loss, e.tol_loss, torch.float32)
     close(lse.detach(), e.lse, e.tol_lse, torch.float32)
-    g = torch.full((8,), 100.0, device="cuda")
+    g = torch.full((8 * copies,), 100.0, device="cuda")
     want, tol = e.grad(g)
     got, = torch.autograd.grad(loss, leaf, g)
     close(got, want, tol, dtype)
     close(K.distill_rows_grad(z, idx, val, g)[2], want, tol, dtype)
-    assert not got[1, 5:2900].any()
+    assert not got[1::8, 5:2900].any()
 
 
-def test_rows_that_are_not_numbers():
+@pytest.mark.parametrize("vocab,copies", [(5001, 1), (1501, 200)])
+def test_rows_that_are_not_numbers(vocab, copies):
     """NaN and infinities stay in their rows, and rows without a teacher take none of them."""
     from zotitan_b200 import kernels as K
-    z, idx, val = make(10, 5001, 12, torch.float32, seed=6, empty=False)
-    ones = torch.ones(10, device="cuda")
+    z, idx, val = make(10, vocab, 12, torch.float32, seed=6, empty=False)
+    ones = torch.ones(10 * copies, device="cuda")
 
-    def both_ways():   # each entry point adds a row up in its own order
-        leaf = z.detach().clone().requires_grad_()
-        loss, lse = K.distill_rows(leaf, idx, val)
-        return (loss.detach(), lse.detach(), *torch.autograd.grad(loss, leaf, ones)), K.distill_rows_grad(z, idx, val, ones)
+    def both_ways():   # each entry point adds a row up in its own order; the last ten rows
+        zz, ii, vv = (t.repeat(copies, 1) for t in (z, idx, val))
+        leaf = zz.detach().requires_grad_()
+        loss, lse = K.distill_rows(leaf, ii, vv)
+        a = (loss.detach(), lse.detach(), *torch.autograd.grad(loss, leaf, ones))
+        return [[t[-10:] for t in r] for r in (a, K.distill_rows_grad(zz, ii, vv, ones))]
 
     clean = both_ways()
-    z[0, 4000] = math.nan
+    z[0, 1400] = math.nan
     z[1, 7] = math.inf
     z[2] = -math.inf
-    idx[3, 4] = 5001                                  # beyond the vocabulary
+    idx[3, 4] = vocab                                 # beyond the vocabulary
     val[4, 2] = math.nan
     val[5, 0] = math.inf
     z[6, idx[6, 1]] = -math.inf                       # mass on an impossible token
@@ -592,10 +610,11 @@ def test_differentiable_once():
 def test_padded_batch():
     """Most rows without a teacher, their logits NaN: zeros there, the others as on their own."""
     from zotitan_b200 import kernels as K
-    for dt, vocab, shift in (("bf16", 30001, 0), ("f32", 9001, 1), ("f16", 5003, 3)):
-        z, idx, val = make(400, vocab, 8, DTYPES[dt], seed=15, empty=False, shift=shift)
-        w = torch.rand(400, device="cuda")
-        keep = torch.arange(400, device="cuda") % 5 == 2
+    for dt, rows, vocab, shift in (("bf16", 400, 30001, 0), ("f32", 400, 9001, 1), ("f16", 400, 5003, 3), ("bf16", 1500, 1003, 1),
+                                   ("f32", 320, 40001, 0)):
+        z, idx, val = make(rows, vocab, 8, DTYPES[dt], seed=15, empty=False, shift=shift)
+        w = torch.rand(rows, device="cuda")
+        keep = torch.arange(rows, device="cuda") % 5 == 2
         alone = K.distill_rows_grad(z[keep].contiguous(), idx[keep], val[keep], w[keep])
         z[~keep], idx[~keep] = math.nan, -1
         leaf = z.detach().requires_grad_()
@@ -612,21 +631,22 @@ def test_padded_batch():
         close(alone[0], e.loss, e.tol_loss, torch.float32)
 
 
-def test_large_biases():
+@COPIES
+def test_large_biases(copies):
     """Logits far from zero: the common part cancels in loss and gradient (16-bit logits that far
     apart are exact inputs all the same)."""
     from zotitan_b200 import kernels as K
     for dt, shift in (("f32", 3000.0), ("f32", 726817.0), ("f32", 1e7), ("f32", -1e20), ("f16", -2000.0), ("bf16", 1e4), ("f32", 2e30)):
         dtype = DTYPES[dt]
         z, idx, val = make(6, 2000, 9, dtype, seed=16, empty=False)
-        z = (z.float() + shift).to(dtype)
+        z, idx, val = ((t.repeat(copies, 1)) for t in ((z.float() + shift).to(dtype), idx, val))
         e = Exact(z, idx, val, 1.0)
         leaf = z.detach().requires_grad_()
         loss, lse = K.distill_rows(leaf, idx, val)
         # mc = round(m log2 e) is the same for every term; its own rounding shows in lse alone
         close(loss.detach(), e.loss, e.tol_loss, torch.float32)
         close(lse.detach(), e.lse, e.tol_lse, torch.float32)
-        g = torch.full((6,), 64.0, device="cuda")
+        g = torch.full((6 * copies,), 64.0, device="cuda")
         want, tol = e.grad(g)
         got, = torch.autograd.grad(loss, leaf, g)
         close(got, want, tol, dtype)
