@@ -718,6 +718,27 @@ def test_captured_before_any_other_call():
     assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
 
 
+@pytest.mark.parametrize("V", [1000, 1003])
+def test_gradient_room_of_one_position_a_sequence(V):
+    """Rows a whole sequence apart: the gradient takes the room of its rows, not of the sequences."""
+    from zotitan_b200 import kernels as K
+    z, idx, val = make(4, V, 6, torch.bfloat16, seed=18, empty=False)
+    whole = torch.zeros(4, 50, V, dtype=torch.bfloat16, device="cuda")
+    whole[:, -1] = z
+    last = whole[:, -1].detach()
+    g = torch.full((4,), 64.0, device="cuda")
+    e = Exact(z, idx, val, 1.0)
+    want, tol = e.grad(g)
+    leaf = last.clone().requires_grad_()
+    loss, _ = K.distill_rows(leaf.as_strided(last.shape, (V, 1)), idx, val)
+    strided = last.requires_grad_()
+    loss2, _ = K.distill_rows(strided, idx, val)
+    for got in (torch.autograd.grad(loss, leaf, g)[0], torch.autograd.grad(loss2, strided, g)[0],
+                K.distill_rows_grad(last.detach(), idx, val, g)[2]):
+        close(got, want, tol, torch.bfloat16)
+        assert got.untyped_storage().nbytes() <= 4 * (V + 8) * 2
+
+
 def test_refusals():
     from zotitan_b200 import kernels as K
     z, idx, val = make(8, 500, 6, torch.bfloat16, seed=12)

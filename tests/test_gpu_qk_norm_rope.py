@@ -294,6 +294,11 @@ def test_refusals():
         K.qk_norm_rope_(q, q, wq, wk, cos, sin)
     with pytest.raises(ValueError, match="overlap"):
         K.qk_norm_rope_(q[:, :, :2], q[:, :, 1:3], wq, wk, cos, sin)
+    # every stride holds a position's q and k, but a position of one batch row reaches another's k
+    store = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    lying = [store.as_strided((2, 2, 1, 64), (192, 128, 64, 1), at) for at in (0, 64)]
+    with pytest.raises(ValueError, match="overlap"):
+        K.qk_norm_rope_(*lying, wq, wk, cos[:, :2], sin[:, :2])
     K.qk_norm_rope_(q[:, :, :2], q[:, :, 2:], wq, wk, cos, sin)
     with pytest.raises(ValueError, match="twice"):
         K.qk_norm_rope_(q[:1].expand(2, -1, -1, -1), k, wq, wk, cos, sin)

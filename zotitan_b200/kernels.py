@@ -1101,11 +1101,15 @@ def qk_norm_rope_(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
         if any(_overlap(t, o) for o in (q_weight, k_weight, cos, sin)):
             raise ValueError(f"{name} overlaps a weight or a table")
     if _overlap(q4, k4):
-        # slices of the same rows: equal position strides, disjoint inside a position
-        rows = [(d, q4.stride(d)) for d in (0, 1) if q4.shape[d] > 1]
+        # slices of the same rows: equal position strides, disjoint inside a position, and positions
+        # that hold both are disjoint too
         spans = [(t.data_ptr() // t.element_size(), (t.shape[2] - 1) * t.stride(2) + t.shape[3]) for t in (q4, k4)]
         (a, na), (b, nb) = sorted(spans)
-        if (any(k4.stride(d) != s or s < b + nb - a for d, s in rows) or a + na > b):
+        need, apart = b + nb - a, a + na <= b
+        for s, other, n in sorted((q4.stride(d), k4.stride(d), q4.shape[d]) for d in (0, 1) if q4.shape[d] > 1):
+            apart = apart and s == other and s >= need
+            need += s * (n - 1)
+        if not apart:
             raise ValueError("q and k overlap in memory")
     for t in (q, k):
         if not t.is_inference():
@@ -1154,6 +1158,13 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])
 
 
+def _grad_of(x: torch.Tensor) -> torch.Tensor:
+    """Room for the gradient of x: rows aligned as x's are, with less than a row between them (x may
+    be one position of every sequence, whose row stride is a whole sequence)."""
+    vocab = x.shape[1]
+    return x.new_empty_strided(x.shape, (vocab + (_ld(x) - vocab) % 8, 1))   # 8 elements: 16 or 32 bytes
+
+
 def _distill_call(entry, x, top_idx, top_logits, temperature, grad=None, weight=None, weight_lse=None, loss=0, lse=0, stats=0):
     rows, vocab = x.shape
     device = x.device
@@ -1189,8 +1200,7 @@ def _distill_backward(ctx, g, g_lse):
     if g is None and g_lse is None:
         return None, None, None, None
     x, top_idx, top_logits, stats = ctx.saved_tensors
-    # the logits' own row stride: rows keep their alignment
-    grad = x.new_empty_strided(x.shape, (_ld(x), 1))
+    grad = _grad_of(x)
     _distill_call("zt_distill_rows_backward", x, top_idx, top_logits, ctx.temperature, grad=grad,
                   weight=g.contiguous() if g is not None else None,
                   weight_lse=g_lse.contiguous() if g_lse is not None else None, stats=stats.data_ptr())
@@ -1237,7 +1247,7 @@ def distill_rows_grad(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: t
         _same_device(device, weight=weight)
     x = _rows_of(logits)
     if out is None:
-        out = x.new_empty_strided(x.shape, (_ld(x), 1))
+        out = _grad_of(x)
     else:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != device:
             raise ValueError("out must have the logits' shape, dtype and device")
