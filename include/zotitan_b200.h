@@ -659,7 +659,8 @@ typedef struct zt_linear_distill_args {
  * a bad shape. */
 ZT_API size_t zt_linear_distill_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int32_t top);
 ZT_API int zt_linear_distill(const zt_linear_distill_args* args, void* stream);
-/* The device error flag of the GEMM's bounded waits (0: none); reading clears it. */
+/* The device error flag of the GEMM's bounded waits (0: none); reading clears it. After an
+ * expired wait the rows that the GEMM did not finish are NaN, those without a teacher 0. */
 ZT_API int zt_linear_distill_take_error(int32_t* code);
 
 /* ---- query / key norms with the rotary embedding ------------------------------------- */

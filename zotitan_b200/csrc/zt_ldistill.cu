@@ -21,7 +21,8 @@
 //    and pick theirs out by index.
 // 3. combine_kernel: a row's sums over the splits, then its list.
 // Every mbarrier wait is bounded; on expiry the kernel records an error
-// (zt_linear_distill_take_error), drains its own copies and MMAs and frees its tensor memory.
+// (zt_linear_distill_take_error), drains its own copies and MMAs, frees its tensor memory and leaves
+// NaN for every sum that it did not finish.
 #include <math.h>
 
 #include "zt_distill.cuh"
@@ -236,10 +237,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t leader_acce0 = peer_addr(&acce[0], 0), leader_acce1 = peer_addr(&acce[1], 0);
     uint32_t tcount = 0;
     bool ok = true;
-    for (int item = cid; ok && item < n_items; item += ncl) {
+    for (int item = cid; item < n_items; item += ncl) {
       int mt, split, nt0, nt1;
       item_range(P, item, mt, split, nt0, nt1);
       const int row = mt * kTile + (int)rank * (int)kHalfRows + row_local;
+      if (!ok) {   // a wait has expired: what is left of the queue is not a number
+        if (row < P.rows) P.partials[(size_t)(2 * split + half) * P.rows_pad + row] = make_float2(-INFINITY, NAN);
+        continue;
+      }
       // the row's entries of this half's columns, from this split's first column on
       const int32_t* list = P.idx + (int64_t)row * P.top;
       float* z = P.z + (int64_t)row * P.top;
@@ -340,7 +345,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
       }
-      if (ok && row < P.rows) P.partials[(size_t)(2 * split + half) * P.rows_pad + row] = make_float2(st.m, st.s);
+      if (row < P.rows) P.partials[(size_t)(2 * split + half) * P.rows_pad + row] = make_float2(st.m, ok ? st.s : NAN);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");   // no copy is in flight when the thread leaves
   }
