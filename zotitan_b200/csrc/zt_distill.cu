@@ -229,7 +229,7 @@ template <int S> struct Shared {
   unsigned long long list[kMaxTop * List::kBytes / 8];
   Stat red[S / 32];   // the warps' sums
   Stat mine, total;   // this CTA's, the row's
-  int none, bad;      // no teacher: the row's logits need not be read; an index that does not exist
+  int none, bad;      // no teacher: the row's logits need not be read; a list that makes the row NaN
 };
 
 // The list's warp: the row's finished sum from the stream warps' and, over the cluster, the
@@ -267,8 +267,8 @@ __device__ __forceinline__ void leave(int parts) {
   if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// (m, s) of a row's finished sum as it is kept: no finite logit, or an index that does not
-// exist, makes the row NaN.
+// (m, s) of a row's finished sum as it is kept: no finite logit, or a list with an index that does not
+// exist or a value that is no number, makes the row NaN.
 __device__ __forceinline__ Stat final_stat(Stat st, bool bad) {
   if (bad || st.m == -INFINITY) st.s = NAN;
   return st;

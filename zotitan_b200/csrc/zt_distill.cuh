@@ -156,7 +156,7 @@ __host__ __device__ inline int list_capacity(int top) {
 
 struct Teacher {
   bool any;   // the row has a teacher
-  bool bad;   // an index >= vocab
+  bool bad;   // an index >= vocab, or a value that is NaN or +inf, on an entry with mass: the row is NaN
 };
 
 // The loads of four entries a lane are on their way before the first is looked at.
@@ -180,7 +180,7 @@ __device__ __forceinline__ Teacher read_list(const List& s, const I* __restrict_
         const float f = (float)v[e];
         const bool on = i[e] >= 0 && !(f == -INFINITY);
         some = some || on;
-        out = out || (on && (int64_t)i[e] >= vocab);
+        out = out || (on && ((int64_t)i[e] >= vocab || !(f < INFINITY)));
         s.idx[k0 + 32 * e] = on && (int64_t)i[e] < vocab ? (int32_t)i[e] : -1;
         s.p[k0 + 32 * e] = on ? f : -INFINITY;
       }

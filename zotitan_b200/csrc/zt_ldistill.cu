@@ -50,7 +50,7 @@ static_assert((kTile / 2) << kHalfShift == (int)0x80000000, "the half's bit lead
 constexpr size_t kSmem = 1024 + kStages * kStageBytes + 256 + (kWindow + kSlab) * 32 * kEpilogueWarps * 4;
 constexpr uint32_t kIdesc = idesc_bf16(256, 256);
 constexpr int kListWarps = 8;
-enum { kHasTeacher = 0, kNoTeacher = 1, kBadIndex = 2 };
+enum { kHasTeacher = 0, kNoTeacher = 1, kBadList = 2 };
 
 __device__ int g_distill_error = 0;
 
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(32 * kListWarps) list_kernel(const __grid_cons
     }
     first += __popc(__ballot_sync(0xffffffffu, key < 0x80000000u));
   }
-  if (lane == 0) P.status[row] = first << 2 | (!t.any ? kNoTeacher : t.bad ? kBadIndex : kHasTeacher);
+  if (lane == 0) P.status[row] = first << 2 | (!t.any ? kNoTeacher : t.bad ? kBadList : kHasTeacher);
 }
 
 __device__ __forceinline__ void item_range(const Params& P, int item, int& mt, int& split, int& nt0, int& nt1) {
@@ -415,8 +415,8 @@ __global__ void __launch_bounds__(32 * kListWarps) combine_kernel(const __grid_c
   }
   a = warp_sum(a) * (kLn2 * P.temperature * P.temperature);
   if (lane == 0) {
-    P.loss[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : a;
-    P.lse[row] = status == kNoTeacher ? 0.f : status == kBadIndex ? NAN : sum_lse(st, P.c, P.temperature);
+    P.loss[row] = status == kNoTeacher ? 0.f : status == kBadList ? NAN : a;
+    P.lse[row] = status == kNoTeacher ? 0.f : status == kBadList ? NAN : sum_lse(st, P.c, P.temperature);
   }
 }
 

@@ -1217,8 +1217,8 @@ def distill_rows(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.
     With T the temperature, q = softmax(logits / T) and p = softmax(top_logits / T) over the
     list, returns (loss, lse) fp32 [rows]:
       loss = T^2 sum_k p_k (log p_k - log q[top_idx_k]),  lse = logsumexp(logits / T),
-    both 0 on rows without an entry and differentiable (once) in the logits. An index >= vocab
-    makes its row NaN."""
+    both 0 on rows without an entry and differentiable (once) in the logits. An index >= vocab, or
+    a teacher's value that is NaN or +inf, makes its row NaN."""
     device = _check_logits(logits)
     temperature = float(temperature)
     top_idx, top_logits = _check_list(logits.shape[0], device, top_idx, top_logits, temperature)
