@@ -11,6 +11,7 @@ from dataclasses import dataclass, field
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib as L
 
@@ -552,6 +553,7 @@ def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
 def eggroll_rope_(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, seq: int, head_dim: int):
     """In-place rotary embedding of q [rows, Hq*hd] and k [rows, Hk*hd] (bf16, row r at
     position r % seq) with cos, sin [seq, hd] bf16 (zt_eggroll_rope)."""
+    _plain_call("eggroll_rope_", q, k, cos, sin)
     for t, name in ((q, "q"), (k, "k"), (cos, "cos"), (sin, "sin")):
         _check_cuda(t, name)
         if t.dtype != torch.bfloat16 or not t.is_contiguous():
@@ -948,6 +950,16 @@ def _raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _plain_call(name: str, *tensors):
+    """Refuses what a launch would answer wrongly without a word: inputs with a forward-mode tangent
+    (the results would have none, and a tensor written in place would keep its own), and a trace
+    (it would hold the allocation of the outputs and no launch)."""
+    if torch._C._is_tracing():
+        raise ValueError(f"{name} cannot be traced")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{name} has no forward-mode derivative")
+
+
 def _same_device(device: torch.device, **others):
     for name, t in others.items():
         if t.device != device:
@@ -1050,6 +1062,7 @@ class _QkNormRope(torch.autograd.Function):
 
 def _qk_backward(ctx, gq, gk):
     q, k, wq, wk, cos, sin = ctx.saved_tensors
+    _plain_call("qk_norm_rope's backward", gq, gk, q, k, wq, wk)
     gq, gk = _unit(gq), _unit(gk)
     hd = q.shape[-1]
     dq, dk, dw = q.new_empty(q.shape), k.new_empty(k.shape), wq.new_empty((2, hd))
@@ -1074,7 +1087,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     head_dim] (an optional leading batch; any strides, a fused projection's slices among
     them), norm weights [head_dim], cos and sin [positions, head_dim], [1, ...] or [batch, ...]
     (the halves of a head rotate against each other). fp32 inside, one rounding: returns new
-    contiguous (q, k). Differentiable once in q, k and the weights (sums in a fixed order)."""
+    contiguous (q, k). Differentiable once in q, k and the weights (sums in a fixed order), by
+    backward passes alone: forward-mode tangents and traces are refused, here and below."""
+    _plain_call("qk_norm_rope", q, k, q_weight, k_weight, cos, sin)
     q4, k4, cos, sin, own_rows = _check_qk(q, k, q_weight, k_weight, cos, sin)
     eps = float(eps)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
@@ -1090,6 +1105,7 @@ def qk_norm_rope_(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
                   sin: torch.Tensor, eps: float = 1e-6):
     """qk_norm_rope in place on q and k, which need unit stride inside a head and must not
     share elements (slices of one fused projection do not); not differentiable."""
+    _plain_call("qk_norm_rope_", q, k, q_weight, k_weight, cos, sin)
     q4, k4, cos, sin, own_rows = _check_qk(q, k, q_weight, k_weight, cos, sin)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
         raise ValueError("qk_norm_rope_ is not differentiable: use qk_norm_rope")
@@ -1200,6 +1216,7 @@ def _distill_backward(ctx, g, g_lse):
     if g is None and g_lse is None:
         return None, None, None, None
     x, top_idx, top_logits, stats = ctx.saved_tensors
+    _plain_call("distill_rows' backward", g, g_lse, x)
     grad = _grad_of(x)
     _distill_call("zt_distill_rows_backward", x, top_idx, top_logits, ctx.temperature, grad=grad,
                   weight=g.contiguous() if g is not None else None,
@@ -1219,6 +1236,7 @@ def distill_rows(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.
       loss = T^2 sum_k p_k (log p_k - log q[top_idx_k]),  lse = logsumexp(logits / T),
     both 0 on rows without an entry and differentiable (once) in the logits. An index >= vocab, or
     a teacher's value that is NaN or +inf, makes its row NaN."""
+    _plain_call("distill_rows", logits, top_logits)
     device = _check_logits(logits)
     temperature = float(temperature)
     top_idx, top_logits = _check_list(logits.shape[0], device, top_idx, top_logits, temperature)
@@ -1237,6 +1255,7 @@ def distill_rows_grad(logits: torch.Tensor, top_idx: torch.Tensor, top_logits: t
     (zt_distill_rows_grad): returns (loss, lse, grad) with grad[r] = weight[r] dloss_r/dlogits_r
     in the logits' dtype, weight fp32 [rows]. out: where the gradient goes, `logits` itself
     included (then they are gone). Not recorded by autograd."""
+    _plain_call("distill_rows_grad", logits, top_logits, weight, out)
     device = _check_logits(logits)
     temperature = float(temperature)
     rows = logits.shape[0]
@@ -1274,6 +1293,7 @@ def linear_distill(x: torch.Tensor, w: torch.Tensor, top_idx: torch.Tensor, top_
     w [vocab, k] bf16 head weight, the teacher's lists as distill_rows takes them. Returns
     its (loss, lse) on the fp32 products x @ w.T, without writing them. Forward only.
     test_stall_loads / test_wait_cycles: the GEMM loads nothing and reports an expired wait."""
+    _plain_call("linear_distill", x, w, top_logits)
     if not linear_xent_supported(x, w):
         raise ValueError("x and w must be contiguous 16-byte aligned bf16 CUDA matrices with k % 64 == 0")
     (rows, k), vocab, device = x.shape, w.shape[0], x.device
