@@ -1,0 +1,101 @@
+"""Decoders with per-head q/k norms under fuse_llama: calls that the fused forwards have to leave to the
+modules, and what they must not touch."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+
+from test_gpu_distill import model_with_head_norms
+
+pytestmark = pytest.mark.gpu
+
+
+def hidden(seed=1, dtype=torch.bfloat16, shape=(2, 24, 256)):
+    return torch.randn(*shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+
+
+def pair(dtype=torch.bfloat16, seed=0):
+    """The same small model twice, the second with the fused forwards; eager attention, which torch
+    can differentiate forward."""
+    from zotitan_b200.llama_fused import fuse_llama
+    m = model_with_head_norms(seed=seed, layers=1).to(dtype)
+    m.config._attn_implementation = "eager"
+    f = copy.deepcopy(m)
+    fuse_llama(f)
+    return m, f
+
+
+def tables(m, x):
+    return m.model.rotary_emb(x, torch.arange(x.shape[1], device="cuda")[None])
+
+
+PARTS = {"norm": lambda m, x, pe: m.model.norm(x), "attention": lambda m, x, pe: m.model.layers[0].self_attn(x, pe, None)[0],
+         "mlp": lambda m, x, pe: m.model.layers[0].mlp(x)}
+
+
+@pytest.mark.parametrize("no_grad", [True, False])
+@pytest.mark.parametrize("part", PARTS)
+def test_forward_mode(part, no_grad):
+    """Forward-mode derivatives, which torch.no_grad leaves on: those of the modules."""
+    import torch.autograd.forward_ad as fw
+    m, f = pair()
+    x, t = hidden(1), hidden(2)
+    pe = tables(m, x)
+    out = []
+    for model in (m, f):
+        for p in model.parameters():
+            p.requires_grad_(False)
+        with torch.set_grad_enabled(not no_grad), fw.dual_level():
+            out.append(fw.unpack_dual(PARTS[part](model, fw.make_dual(x, t), pe)))
+    assert torch.equal(out[0].primal, out[1].primal)
+    assert out[1].tangent is not None and torch.equal(out[0].tangent, out[1].tangent)
+
+
+def test_forward_mode_in_a_weight():
+    """A tangent on a norm's weight alone, reached through the head norms and the decoder norm."""
+    import torch.autograd.forward_ad as fw
+    m, f = pair()
+    x = hidden(3)
+    pe = tables(m, x)
+    for part, name in (("attention", "model.layers.0.self_attn.q_norm"), ("norm", "model.norm")):
+        out = []
+        for model in (m, f):
+            mod = model.get_submodule(name)
+            w = mod.weight.detach()
+            with torch.no_grad(), fw.dual_level():
+                mod.weight = nn.Parameter(w, requires_grad=False)
+                del mod._parameters["weight"]
+                mod.weight = fw.make_dual(w, torch.ones_like(w))
+                out.append(fw.unpack_dual(PARTS[part](model, x, pe)).tangent.clone())
+                del mod.weight
+                mod.weight = nn.Parameter(w, requires_grad=False)
+        assert torch.equal(out[0], out[1]) and bool(out[1].any())
+
+
+@pytest.mark.parametrize("part", PARTS)
+def test_traced(part):
+    """A trace holds the modules' operations, so it computes on other inputs too."""
+    m, f = pair()
+    x, other = hidden(4), hidden(5)
+    pe = tables(m, x)
+    for p in f.parameters():
+        p.requires_grad_(False)
+    with torch.no_grad():
+        traced = torch.jit.trace(lambda h: PARTS[part](f, h, pe), x, check_trace=False)
+        want = PARTS[part](m, other, pe)
+        assert torch.equal(traced(other), want)
+
+
+@pytest.mark.parametrize("part", PARTS)
+def test_function_transforms(part):
+    """torch.func's gradient and vmap over a fused module: those over the module."""
+    m, f = pair(torch.float32 if part == "attention" else torch.bfloat16)
+    x = hidden(6, m.dtype)
+    pe = tables(m, x)
+    got, want = (torch.func.grad(lambda h: PARTS[part](model, h, pe).float().square().sum())(x) for model in (f, m))
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        both = torch.stack([x, -x])
+        got, want = (torch.func.vmap(lambda h: PARTS[part](model, h, pe))(both) for model in (f, m))
+    assert torch.equal(got, want)
