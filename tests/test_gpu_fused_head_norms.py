@@ -99,3 +99,17 @@ def test_function_transforms(part):
         both = torch.stack([x, -x])
         got, want = (torch.func.vmap(lambda h: PARTS[part](model, h, pe))(both) for model in (f, m))
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("part", PARTS)
+def test_compiled_whole(part, grad):
+    """torch.compile without graph breaks, as over the modules."""
+    m, f = pair()
+    x = hidden(7)
+    pe = tables(m, x)
+    torch._dynamo.reset()
+    with torch.set_grad_enabled(grad):
+        got = torch.compile(lambda h: PARTS[part](f, h, pe), fullgraph=True, backend="eager")(x)
+        assert torch.equal(got, PARTS[part](m, x, pe))
+    torch._dynamo.reset()

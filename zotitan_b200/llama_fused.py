@@ -32,8 +32,8 @@ RMSNorm and MLP and an attention of their own:
 Each other fused forward defers to the module's own forward when gradients are enabled,
 the activations are not bf16 on a CUDA device, the layout does not fit (head_dim not a
 multiple of 16, per-sequence position ids), or the MLP's activation is not SiLU. All of them
-do where torch itself has to follow the operations: under forward-mode derivatives, in a trace
-and inside torch.func's transforms.
+do where torch itself has to follow the operations: under forward-mode derivatives, in a trace,
+inside torch.func's transforms and, those of decoders with head norms, under torch.compile.
 `unfuse_llama(model)` restores the original forwards.
 """
 from __future__ import annotations
@@ -67,10 +67,10 @@ def assume_causal():
 
 def _torch_must_see(m: nn.Module) -> bool:
     """Calls whose operations torch itself follows, which a kernel launch hides from it: forward-mode
-    derivatives (torch.no_grad leaves them on), traces, torch.func's transforms. Under
-    torch.compile the fused forwards break the graph and run as they do outside of it."""
+    derivatives (torch.no_grad leaves them on), traces, torch.func's transforms. And torch.compile for
+    decoders with head norms; fused Llama forwards break its graph and run as they do outside of it."""
     if torch.compiler.is_compiling():
-        return False
+        return type(m).__name__.startswith("Qwen3")
     return (forward_ad._current_level >= 0 or torch._C._is_tracing()
             or torch._C._functorch.peek_interpreter_stack() is not None)
 
