@@ -113,3 +113,20 @@ def test_compiled_whole(part, grad):
         got = torch.compile(lambda h: PARTS[part](f, h, pe), fullgraph=True, backend="eager")(x)
         assert torch.equal(got, PARTS[part](m, x, pe))
     torch._dynamo.reset()
+
+
+def test_trainable_frequencies():
+    """A rotary embedding whose frequencies are trained: the gradient of cos and sin is the modules'."""
+    m, f = pair(torch.float32)
+    x = hidden(8, torch.float32)
+    grads = []
+    for model in (m, f):
+        freq = model.model.rotary_emb.inv_freq.detach().clone().requires_grad_()
+        ang = torch.arange(x.shape[1], device="cuda")[:, None] * freq
+        ang = torch.cat((ang, ang), -1)[None]
+        out = model.model.layers[0].self_attn(x, (ang.cos(), ang.sin()), None)[0]
+        grads.append(torch.autograd.grad(out.square().sum(), freq)[0])
+    assert torch.equal(*grads) and bool(grads[0].any())
+    with torch.no_grad():     # the same tables in an evaluation
+        outs = [model.model.layers[0].self_attn(x, (ang.cos().requires_grad_(), ang.sin().requires_grad_()), None)[0] for model in (m, f)]
+    assert torch.equal(*outs)

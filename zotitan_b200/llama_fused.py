@@ -134,7 +134,8 @@ def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, at
     if (not hidden_states.is_cuda or dt not in (torch.bfloat16, torch.float16, torch.float32) or cos is None
             or hidden_states.dim() != 3 or hidden_states.numel() == 0 or cos.dim() != 3
             or cos.shape[0] not in (1, hidden_states.shape[0]) or cos.shape[1:] != (hidden_states.shape[1], hd) or hd % 2
-            or hd > 512 or eps != self.k_norm.variance_epsilon or wq.dtype != wk.dtype or wq.dtype not in (dt, torch.float32) or cos.dtype not in (dt, torch.float32)
+            or hd > 512 or eps != self.k_norm.variance_epsilon or wq.dtype != wk.dtype or wq.dtype not in (dt, torch.float32)
+            or cos.dtype not in (dt, torch.float32) or cos.requires_grad or sin.requires_grad   # trained frequencies
             or torch.is_autocast_enabled("cuda")):
         return self._zt_orig_forward(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
     from transformers.models.qwen3.modeling_qwen3 import ALL_ATTENTION_FUNCTIONS, eager_attention_forward
