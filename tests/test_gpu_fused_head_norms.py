@@ -130,3 +130,83 @@ def test_trainable_frequencies():
     with torch.no_grad():     # the same tables in an evaluation
         outs = [model.model.layers[0].self_attn(x, (ang.cos().requires_grad_(), ang.sin().requires_grad_()), None)[0] for model in (m, f)]
     assert torch.equal(*outs)
+
+
+class Keep(nn.Module):
+    """A projection that hands out a tensor it goes on holding."""
+
+    def __init__(self, out):
+        super().__init__()
+        self.out = out
+
+    def forward(self, x):
+        return self.out
+
+
+def llama_attention():
+    from transformers import LlamaConfig, LlamaForCausalLM
+    from zotitan_b200.llama_fused import fuse_llama
+    cfg = LlamaConfig(vocab_size=100, hidden_size=256, intermediate_size=512, num_hidden_layers=1, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=64, attn_implementation="sdpa")
+    torch.manual_seed(0)
+    m = LlamaForCausalLM(cfg).to("cuda", torch.bfloat16).eval()
+    fuse_llama(m)
+    return m
+
+
+@pytest.mark.parametrize("how", ["hook", "every_module_hook", "adapter_hook", "base_hook", "module"])
+@pytest.mark.parametrize("llama", [False, True])
+def test_projection_outputs_that_others_hold(how, llama):
+    """What a hook took from a projection, or a projection holds itself, stays as it was."""
+    from zotitan_b200.lora import LoRALinear
+    f = llama_attention() if llama else pair()[1]
+    x = hidden(9)
+    pe = tables(f, x)
+    attn = f.model.layers[0].self_attn
+    if "hook" in how and how.split("_")[0] in ("adapter", "base"):
+        for name in ("q_proj", "k_proj"):
+            setattr(attn, name, LoRALinear(getattr(attn, name), 8, 16).cuda())
+    with torch.inference_mode():
+        q, k = attn.q_proj(x), attn.k_proj(x)
+        want = attn(x, pe, None)[0]
+        seen = {}
+        handles = []
+        if how in ("hook", "adapter_hook", "base_hook"):
+            for name in ("q_proj", "k_proj"):
+                mod = getattr(attn, name)
+                if how == "base_hook":
+                    mod.lora_A.weight.zero_()     # lora_B is zero: nothing is added to what the base gives out
+                    mod = mod.base_linear
+                handles.append(mod.register_forward_hook(lambda mod, a, out, name=name: seen.__setitem__(name, out)))
+        elif how == "every_module_hook":
+            names = {attn.q_proj: "q_proj", attn.k_proj: "k_proj"}
+            handles.append(nn.modules.module.register_module_forward_hook(
+                lambda mod, a, out: seen.__setitem__(names[mod], out) if mod in names else None))
+        else:
+            seen = {"q_proj": q.clone(), "k_proj": k.clone()}
+            attn.q_proj, attn.k_proj = Keep(seen["q_proj"]), Keep(seen["k_proj"])
+        got = attn(x, pe, None)[0]
+        for h in handles:
+            h.remove()
+    assert torch.equal(seen["q_proj"], q) and torch.equal(seen["k_proj"], k)
+    if llama or how != "every_module_hook":     # the hook for every module is also the norms': those run themselves
+        assert torch.equal(got, want)
+
+
+def test_projections_that_share_memory():
+    """Query and key heads that a projection gives out as the same memory, or one head for all."""
+    m, f = pair()
+    x = hidden(10)
+    pe = tables(m, x)
+    q = hidden(11, shape=(2, 24, 384))
+    one = hidden(12, shape=(2, 24, 64))
+    for key in (q[..., :128], one.unsqueeze(2).expand(-1, -1, 2, -1)):
+        out = []
+        with torch.no_grad():
+            for model in (m, f):
+                attn = model.model.layers[0].self_attn
+                attn.q_proj, attn.k_proj = Keep(q.clone()), Keep(None)
+                attn.k_proj.out = attn.q_proj.out[..., :128] if key.dim() == 3 else key
+                out.append(attn(x, pe, None)[0].float())
+        scale = float(out[0].square().mean().sqrt())     # as in test_gpu_distill.test_attention_with_head_norms
+        assert float((out[0] - out[1]).square().mean().sqrt()) <= 0.02 * scale

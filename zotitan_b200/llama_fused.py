@@ -11,8 +11,8 @@ LlamaMLP instance of a model for one that calls this package's kernels:
   weight product): LlamaRMSNorm.forward with its rounding points; only the summation
   order of a row's squares differs.
 - attention: the q/k/v projections (the modules themselves, so LoRA wrappers keep
-  working), the rotary embedding applied in place on the projection outputs by
-  `zt_eggroll_rope` (bit-exact with apply_rotary_pos_emb), the configured attention
+  working), the rotary embedding applied in place on the projection outputs (on copies
+  where a hook or another module may hold them) by `zt_eggroll_rope` (bit-exact with apply_rotary_pos_emb), the configured attention
   implementation called as LlamaAttention.forward calls it, then o_proj.
 - MLP: for plain bias-free bf16 linears and rows in 256-row tiles, gate, up and the
   SwiGLU as one tcgen05 GEMM (`zt_gemm_swiglu`, the SwiGLU in its epilogue); otherwise
@@ -25,9 +25,9 @@ RMSNorm and MLP and an attention of their own:
 
 - attention with head norms: both norms and the rotary embedding in one pass over the
   projection outputs, in place (`zt_qk_norm_rope`; fp32 inside, rounded once where the
-  modules round after the norm, its weight, each rotary product and their sum). With
-  gradients enabled the same kernel runs out of place and brings its backward
-  (`kernels.qk_norm_rope`), in bf16, fp16 or fp32.
+  modules round after the norm, its weight, each rotary product and their sum). Where others
+  may hold the outputs the same kernel runs out of place; so it does with gradients enabled,
+  and brings its backward (`kernels.qk_norm_rope`), in bf16, fp16 or fp32.
 
 Each other fused forward defers to the module's own forward when gradients are enabled,
 the activations are not bf16 on a CUDA device, the layout does not fit (head_dim not a
@@ -46,6 +46,7 @@ import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 
 from . import kernels as K
+from .lora import LoRALinear
 
 
 _ASSUME_CAUSAL = False
@@ -79,6 +80,18 @@ def _fast(m: nn.Module, x: torch.Tensor) -> bool:
     return (not torch.is_grad_enabled()) and x.is_cuda and x.dtype == torch.bfloat16 and not _torch_must_see(m)
 
 
+def _unhooked(m: nn.Module) -> bool:
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
+def _ours(m: nn.Module) -> bool:
+    """Whether the output of a projection is nobody else's and may be overwritten: a linear's (of an
+    adapter too) that no hook has seen."""
+    if type(m) is LoRALinear and _unhooked(m):
+        m = m.base_linear
+    return type(m) is nn.Linear and _unhooked(m) and not torch.nn.modules.module._has_any_global_hook()
+
+
 def _rmsnorm_forward(self, hidden_states):
     w = self.weight
     if (not _fast(self, hidden_states) or w.dtype != torch.bfloat16 or hidden_states.shape[-1] % 8
@@ -99,8 +112,8 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
     q = self.q_proj(hidden_states)
     k = self.k_proj(hidden_states)
     v = self.v_proj(hidden_states)
-    q = q if q.is_contiguous() else q.contiguous()
-    k = k if k.is_contiguous() else k.contiguous()
+    q = q if q.is_contiguous() and _ours(self.q_proj) else q.clone(memory_format=torch.contiguous_format)
+    k = k if k.is_contiguous() and _ours(self.k_proj) else k.clone(memory_format=torch.contiguous_format)
     # rows of q / k are tokens at positions 0..T-1 of each sequence (cos[0] is shared)
     K.eggroll_rope_(q, k, cos[0].contiguous(), sin[0].contiguous(), T, hd)
     q = q.view(bsz, T, -1, hd).transpose(1, 2)
@@ -118,8 +131,7 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
 
 def _plain_norm(m, hd: int) -> bool:
     """A head norm as the model built it: nothing hooked onto it that the fused pass would skip."""
-    return (type(m).__name__ == "Qwen3RMSNorm" and m.weight.shape == (hd,) and not m._forward_hooks
-            and not m._forward_pre_hooks and not m._backward_hooks and not m._backward_pre_hooks)
+    return type(m).__name__ == "Qwen3RMSNorm" and m.weight.shape == (hd,) and _unhooked(m)
 
 
 def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None,
@@ -143,7 +155,8 @@ def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, at
     q = self.q_proj(hidden_states).view(bsz, T, -1, hd)
     k = self.k_proj(hidden_states).view(bsz, T, -1, hd)
     v = self.v_proj(hidden_states).view(bsz, T, -1, hd).transpose(1, 2)
-    norm = K.qk_norm_rope if torch.is_grad_enabled() else K.qk_norm_rope_
+    in_place = not torch.is_grad_enabled() and _ours(self.q_proj) and _ours(self.k_proj)
+    norm = K.qk_norm_rope_ if in_place else K.qk_norm_rope
     q, k = norm(q, k, wq, wk, cos, sin, eps)
     q, k = q.transpose(1, 2), k.transpose(1, 2)
     if past_key_values is not None:
