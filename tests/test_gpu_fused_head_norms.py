@@ -210,3 +210,30 @@ def test_projections_that_share_memory():
                 out.append(attn(x, pe, None)[0].float())
         scale = float(out[0].square().mean().sqrt())     # as in test_gpu_distill.test_attention_with_head_norms
         assert float((out[0] - out[1]).square().mean().sqrt()) <= 0.02 * scale
+
+
+@pytest.mark.parametrize("llama", [False, True])
+def test_hooked_projections_of_the_mlp_run(llama):
+    """Hooks on gate, up and the activation see their calls, at the sizes of the fused GEMM too."""
+    from zotitan_b200.llama_fused import fuse_llama
+    m, f = pair()
+    mlp = f.model.layers[0].mlp
+    if llama:
+        from transformers import LlamaConfig
+        from transformers.models.llama.modeling_llama import LlamaMLP
+        mlp = LlamaMLP(LlamaConfig(hidden_size=256, intermediate_size=512)).to("cuda", torch.bfloat16)
+        fuse_llama(mlp)
+    x = hidden(13, shape=(2, 128, 256))
+    with torch.no_grad():
+        want = mlp(x)
+        seen = []
+        for mod in (mlp.gate_proj, mlp.up_proj, mlp.act_fn):
+            h = mod.register_forward_hook(lambda mod, a, out: seen.append(mod))
+            got = mlp(x)
+            h.remove()
+            assert seen == [mod]
+            seen.clear()
+            assert float((got - want).float().square().mean().sqrt()) <= 0.01 * float(want.float().square().mean().sqrt())
+        h = mlp.gate_proj.register_forward_hook(lambda mod, a, out: out * 0)
+        assert not mlp(x).any()
+        h.remove()

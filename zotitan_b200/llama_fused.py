@@ -176,12 +176,12 @@ def is_silu(act) -> bool:
 
 def _plain_linear(m, k: int) -> bool:
     w = getattr(m, "weight", None)
-    return (type(m) is nn.Linear and m.bias is None and w is not None and w.dtype == torch.bfloat16
+    return (type(m) is nn.Linear and _unhooked(m) and m.bias is None and w is not None and w.dtype == torch.bfloat16
             and w.is_contiguous() and w.shape[1] == k)
 
 
 def _mlp_forward(self, x):
-    if not _fast(self, x) or not is_silu(self.act_fn):
+    if not _fast(self, x) or not is_silu(self.act_fn) or not _unhooked(self.act_fn):
         return self._zt_orig_forward(x)
     k = x.shape[-1]
     rows = x.numel() // k
