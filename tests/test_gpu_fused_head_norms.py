@@ -237,3 +237,20 @@ def test_hooked_projections_of_the_mlp_run(llama):
         h = mlp.gate_proj.register_forward_hook(lambda mod, a, out: out * 0)
         assert not mlp(x).any()
         h.remove()
+
+
+def test_hooks_for_every_module_reach_the_head_norms():
+    m, f = pair()
+    x = hidden(14)
+    pe = tables(m, x)
+    attn = f.model.layers[0].self_attn
+    seen = []
+    h = nn.modules.module.register_module_forward_hook(lambda mod, a, out: seen.append(mod))
+    with torch.no_grad():
+        got = attn(x, pe, None)[0]
+    h.remove()
+    assert attn.q_norm in seen and attn.k_norm in seen
+    with torch.no_grad():
+        want = m.model.layers[0].self_attn(x, pe, None)[0]
+    scale = float(want.float().square().mean().sqrt())
+    assert float((got - want).float().square().mean().sqrt()) <= 0.02 * scale

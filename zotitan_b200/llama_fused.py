@@ -81,7 +81,9 @@ def _fast(m: nn.Module, x: torch.Tensor) -> bool:
 
 
 def _unhooked(m: nn.Module) -> bool:
-    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+    """No hook sees a call of m, neither its own nor one for every module."""
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                or torch.nn.modules.module._has_any_global_hook())
 
 
 def _ours(m: nn.Module) -> bool:
@@ -89,7 +91,7 @@ def _ours(m: nn.Module) -> bool:
     adapter too) that no hook has seen."""
     if type(m) is LoRALinear and _unhooked(m):
         m = m.base_linear
-    return type(m) is nn.Linear and _unhooked(m) and not torch.nn.modules.module._has_any_global_hook()
+    return type(m) is nn.Linear and _unhooked(m)
 
 
 def _rmsnorm_forward(self, hidden_states):
