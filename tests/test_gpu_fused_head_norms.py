@@ -254,3 +254,28 @@ def test_hooks_for_every_module_reach_the_head_norms():
         want = m.model.layers[0].self_attn(x, pe, None)[0]
     scale = float(want.float().square().mean().sqrt())
     assert float((got - want).float().square().mean().sqrt()) <= 0.02 * scale
+
+
+class InFp32(nn.Module):
+    def __init__(self, base):
+        super().__init__()
+        self.base = base
+
+    def forward(self, x):
+        return nn.functional.linear(x.float(), self.base.weight.float())
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_projections_in_another_type(grad):
+    """Projections that answer in fp32 to bf16 hidden states: the head norms run as modules there."""
+    m, f = pair()
+    x = hidden(15)
+    pe = tables(m, x)
+    out = []
+    for model in (m, f):
+        attn = model.model.layers[0].self_attn
+        for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
+            setattr(attn, name, InFp32(getattr(attn, name)))
+        with torch.set_grad_enabled(grad):
+            out.append(attn(x, pe, None)[0])
+    assert out[0].dtype == torch.float32 and torch.equal(*out)

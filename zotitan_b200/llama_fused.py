@@ -152,15 +152,18 @@ def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, at
             or cos.dtype not in (dt, torch.float32) or cos.requires_grad or sin.requires_grad   # trained frequencies
             or torch.is_autocast_enabled("cuda")):
         return self._zt_orig_forward(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
-    from transformers.models.qwen3.modeling_qwen3 import ALL_ATTENTION_FUNCTIONS, eager_attention_forward
+    from transformers.models.qwen3.modeling_qwen3 import ALL_ATTENTION_FUNCTIONS, apply_rotary_pos_emb, eager_attention_forward
     bsz, T, _ = hidden_states.shape
     q = self.q_proj(hidden_states).view(bsz, T, -1, hd)
     k = self.k_proj(hidden_states).view(bsz, T, -1, hd)
     v = self.v_proj(hidden_states).view(bsz, T, -1, hd).transpose(1, 2)
-    in_place = not torch.is_grad_enabled() and _ours(self.q_proj) and _ours(self.k_proj)
-    norm = K.qk_norm_rope_ if in_place else K.qk_norm_rope
-    q, k = norm(q, k, wq, wk, cos, sin, eps)
-    q, k = q.transpose(1, 2), k.transpose(1, 2)
+    if type(q) is type(k) is torch.Tensor and q.dtype == k.dtype == dt:
+        in_place = not torch.is_grad_enabled() and _ours(self.q_proj) and _ours(self.k_proj)
+        norm = K.qk_norm_rope_ if in_place else K.qk_norm_rope
+        q, k = norm(q, k, wq, wk, cos, sin, eps)
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+    else:   # projections that answer in a type of their own
+        q, k = apply_rotary_pos_emb(self.q_norm(q).transpose(1, 2), self.k_norm(k).transpose(1, 2), cos, sin)
     if past_key_values is not None:
         k, v = past_key_values.update(k, v, self.layer_idx)
     if _ASSUME_CAUSAL and past_key_values is None and self.sliding_window is None:
