@@ -279,3 +279,30 @@ def test_projections_in_another_type(grad):
         with torch.set_grad_enabled(grad):
             out.append(attn(x, pe, None)[0])
     assert out[0].dtype == torch.float32 and torch.equal(*out)
+
+
+def test_replaced_forwards_are_called():
+    """A forward set on an instance, as offloading and kernel hubs do: before or after fuse_llama, on a norm, a
+    projection or the activation."""
+    from zotitan_b200.llama_fused import fuse_llama, unfuse_llama
+    x = hidden(16, shape=(2, 128, 256))
+    where = {"attention": ("q_norm", "k_norm", "q_proj"), "mlp": ("gate_proj", "up_proj", "act_fn"), "norm": ("",)}
+    for part, names in where.items():
+        for name in names:
+            for before in (True, False):
+                m, f = pair()
+                pe = tables(m, x)
+                out = []
+                for model in (m, f):
+                    root = {"attention": model.model.layers[0].self_attn, "mlp": model.model.layers[0].mlp, "norm": model.model.norm}[part]
+                    mod = root.get_submodule(name)
+                    if before:
+                        unfuse_llama(model)
+                    own = mod.forward
+                    mod.forward = lambda h, own=own: own(h) * 2
+                    if before and model is f:
+                        fuse_llama(model)
+                    with torch.no_grad():
+                        out.append(PARTS[part](model, x, pe).float())
+                scale = float(out[0].square().mean().sqrt())
+                assert float((out[0] - out[1]).square().mean().sqrt()) <= 0.02 * scale, (part, name, before)

@@ -86,12 +86,19 @@ def _unhooked(m: nn.Module) -> bool:
                 or torch.nn.modules.module._has_any_global_hook())
 
 
+def _untouched(m: nn.Module) -> bool:
+    """m runs as its class says: no hook sees it, and its forward is the class's or one that
+    fuse_llama put in that one's place."""
+    return _unhooked(m) and ("forward" not in m.__dict__ or "_zt_orig_forward" in m.__dict__
+                             and getattr(m.__dict__["forward"], "__func__", None) is _FORWARDS[type(m).__name__])
+
+
 def _ours(m: nn.Module) -> bool:
     """Whether the output of a projection is nobody else's and may be overwritten: a linear's (of an
     adapter too) that no hook has seen."""
-    if type(m) is LoRALinear and _unhooked(m):
+    if type(m) is LoRALinear and _untouched(m):
         m = m.base_linear
-    return type(m) is nn.Linear and _unhooked(m)
+    return type(m) is nn.Linear and _untouched(m)
 
 
 def _rmsnorm_forward(self, hidden_states):
@@ -133,7 +140,7 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
 
 def _plain_norm(m, hd: int) -> bool:
     """A head norm as the model built it: nothing hooked onto it that the fused pass would skip."""
-    return type(m).__name__ == "Qwen3RMSNorm" and m.weight.shape == (hd,) and _unhooked(m)
+    return type(m).__name__ == "Qwen3RMSNorm" and m.weight.shape == (hd,) and _untouched(m)
 
 
 def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None,
@@ -181,12 +188,12 @@ def is_silu(act) -> bool:
 
 def _plain_linear(m, k: int) -> bool:
     w = getattr(m, "weight", None)
-    return (type(m) is nn.Linear and _unhooked(m) and m.bias is None and w is not None and w.dtype == torch.bfloat16
+    return (type(m) is nn.Linear and _untouched(m) and m.bias is None and w is not None and w.dtype == torch.bfloat16
             and w.is_contiguous() and w.shape[1] == k)
 
 
 def _mlp_forward(self, x):
-    if not _fast(self, x) or not is_silu(self.act_fn) or not _unhooked(self.act_fn):
+    if not _fast(self, x) or not is_silu(self.act_fn) or not _untouched(self.act_fn):
         return self._zt_orig_forward(x)
     k = x.shape[-1]
     rows = x.numel() // k
@@ -212,11 +219,12 @@ _FORWARDS = {"LlamaRMSNorm": _rmsnorm_forward, "LlamaAttention": _attention_forw
 
 def fuse_llama(model: nn.Module) -> int:
     """Install the fused forwards on every Llama or Qwen3 RMSNorm / attention / MLP module of
-    `model`; returns how many modules were changed. Idempotent."""
+    `model`, but for those whose instances have been given another forward already; returns how
+    many modules were changed. Idempotent."""
     n = 0
     for m in model.modules():
         fn = _FORWARDS.get(type(m).__name__)
-        if fn is None or hasattr(m, "_zt_orig_forward"):
+        if fn is None or hasattr(m, "_zt_orig_forward") or "forward" in m.__dict__:
             continue
         m._zt_orig_forward = m.forward
         m.forward = types.MethodType(fn, m)
@@ -229,7 +237,6 @@ def unfuse_llama(model: nn.Module) -> int:
     n = 0
     for m in model.modules():
         if hasattr(m, "_zt_orig_forward"):
-            m.forward = m._zt_orig_forward
-            del m._zt_orig_forward
+            del m.forward, m._zt_orig_forward   # the class's own again
             n += 1
     return n
