@@ -72,3 +72,57 @@ def test_teacher_that_is_not_a_number_in_the_head(bad):
     for got, was in zip(K.linear_distill(x, w, idx, val), clean):
         assert torch.isnan(got[5]) and torch.isnan(got[299]) and torch.isfinite(got[7])
         assert torch.equal(got[keep], was[keep])
+
+
+def test_frozen_head_keeps_small_probabilities():
+    """Gradients through a frozen fp16 head: hidden rows that pick single columns make the logits exact.
+    One token stands far above the others, whose probabilities of about 2e-9 are below fp16's
+    smallest number, and the teacher agrees; the upstream gradient (a loss scale) makes up for it.
+    The logits' gradient times 2^14 is rounded to fp16: 2^-11 of itself, or 2^-25, half a subnormal
+    step, of 2^-14; the product adds V / 16 + 16 terms of 2 u (tensor cores, as in test_gpu_distill);
+    the result, times g, is rounded once."""
+    from zotitan_b200.losses import head_distill
+    V, d, T = 4096, 64, 1.0
+    gen = torch.Generator(device="cuda").manual_seed(26)
+    w = torch.randn(V, 2 * d, device="cuda", generator=gen) * 0.5     # the first half makes the logits,
+    w[:, :d] -= 5
+    w[:, d:] += 1                                                     # the second sees their gradient,
+    w[17, :d], w[17, d:] = 15.0, 0.0                                  # but for the high token's
+    w = w.half()
+    x = torch.eye(d, 2 * d, device="cuda").half().requires_grad_()
+    idx = torch.tensor([[17, -1]], device="cuda").expand(d, 2)
+    val = torch.zeros(d, 2, device="cuda")
+    g = torch.full((d,), 32768.0, device="cuda")
+    e = Exact(w[:, :d].t(), idx, val, T)
+    dz, tol = e.grad(g)
+    assert float(e.q.median()) < 3e-9
+    want = dz @ w.double()
+    wa = w.double().abs()
+    tol = (tol + 2 ** -11 * dz.abs() + 2 ** -25 * 2 ** -14 * g.double()[:, None]) @ wa
+    tol = tol + (V / 16 + 16) * 2 * U * (dz.abs() @ wa)
+    assert float((tol / want.abs())[:, d:].max()) < 1e-2              # the second half tells
+    loss, _ = head_distill(x, idx, val, w, chunk_rows=48)
+    got, = torch.autograd.grad(loss, x, g)
+    close(got, want, tol, torch.float16)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_frozen_head_rounds_the_result_once(dt):
+    """Upstream gradients that are no powers of two: the hidden gradient is the fp32 product of the
+    logits' rounded gradient with the head (1000 terms: (V / 16 + 16) 2 u on tensor cores, V u
+    elsewhere), times g (u, and u of the product's own store), rounded once to the hidden type."""
+    from zotitan_b200 import kernels as K
+    from zotitan_b200.losses import head_distill
+    dtype, V = DTYPES[dt], 1000
+    x, w, idx, val = operands(300, V, 128, 16, seed=27)
+    x, w = x.to(dtype), w.to(dtype)
+    g = torch.rand(300, device="cuda") + 0.5
+    leaf = x.detach().requires_grad_()
+    loss, _ = head_distill(leaf, idx, val, w, chunk_rows=128)
+    got, = torch.autograd.grad(loss, leaf, g)
+    dz = torch.cat([K.distill_rows_grad(F.linear(c, w), i, v, torch.ones(len(c), device="cuda"))[2]
+                    for c, i, v in zip(x.split(128), idx.split(128), val.split(128))]).double()
+    want = dz @ w.double() * g.double()[:, None]
+    terms = dz.abs() @ w.double().abs() * g.double()[:, None]
+    adds = V * U if dt == "f32" else (V / 16 + 16) * 2 * U
+    close(got, want, adds * terms + 2 * U * want.abs(), dtype)

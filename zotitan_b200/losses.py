@@ -19,6 +19,8 @@ own gradient in place (``zt_distill_rows_grad``).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -111,23 +113,34 @@ def fused_xentropy(model, batch, z_loss_weight: float, compute_accuracy: bool):
 class _FrozenHeadDistill(torch.autograd.Function):
     """head_distill through a head that is not trained: a chunk's logits turn into
     dloss_r/dlogits_r in place and then into dloss_r/dhidden_r, which the backward scales by
-    each row's upstream gradient. lse is not differentiable here."""
+    each row's upstream gradient. lse is not differentiable here.
+
+    Rounded twice, as autograd rounds it that knows the upstream gradient: the logits' gradient
+    to their type, and the result to the hidden type; dloss_r/dhidden_r waits in fp32. In fp16 a
+    probability below 2^-25 would vanish before a loss scale could help, so there the logits'
+    gradient is taken times a power of two, the largest that keeps T (q - p), at most T, below
+    fp16's 65504."""
 
     @staticmethod
     def forward(ctx, hidden, weight, bias, top_idx, top_logits, temperature, chunk_rows):
         R, dev = hidden.shape[0], hidden.device
         loss = torch.empty(R, dtype=torch.float32, device=dev)
         lse = torch.empty(R, dtype=torch.float32, device=dev)
-        dx = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev)
-        ones = torch.ones(min(R, chunk_rows), dtype=torch.float32, device=dev)
+        dx = torch.empty(hidden.shape, dtype=torch.float32, device=dev)
+        scale = 2.0 ** (15 - math.frexp(temperature)[1]) if hidden.dtype == torch.float16 else 1.0
+        scales = torch.full((min(R, chunk_rows),), scale, dtype=torch.float32, device=dev)
         for r0 in range(0, R, chunk_rows):
             r1 = min(R, r0 + chunk_rows)
             logits = F.linear(hidden[r0:r1], weight, bias)
-            loss[r0:r1], lse[r0:r1], grad = K.distill_rows_grad(logits, top_idx[r0:r1], top_logits[r0:r1], ones[:r1 - r0],
+            loss[r0:r1], lse[r0:r1], grad = K.distill_rows_grad(logits, top_idx[r0:r1], top_logits[r0:r1], scales[:r1 - r0],
                                                                 temperature, out=logits)
-            torch.mm(grad, weight, out=dx[r0:r1])
+            if grad.dtype == torch.float32:
+                torch.mm(grad, weight, out=dx[r0:r1])
+            else:
+                torch.mm(grad, weight, out_dtype=torch.float32, out=dx[r0:r1])
             del logits, grad
         ctx.save_for_backward(dx)
+        ctx.rest = scale, hidden.dtype
         ctx.mark_non_differentiable(lse)
         return loss, lse
 
@@ -135,7 +148,9 @@ class _FrozenHeadDistill(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
         dx, = ctx.saved_tensors
-        return (dx * g[:, None]).to(dx.dtype), None, None, None, None, None, None
+        scale, dtype = ctx.rest
+        g = g if scale == 1.0 else g / scale
+        return torch.mul(dx, g[:, None], out=torch.empty_like(dx, dtype=dtype)), None, None, None, None, None, None
 
 
 def head_distill(hidden: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.Tensor, weight: torch.Tensor, bias=None,
