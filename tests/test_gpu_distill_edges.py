@@ -126,3 +126,34 @@ def test_frozen_head_rounds_the_result_once(dt):
     terms = dz.abs() @ w.double().abs() * g.double()[:, None]
     adds = V * U if dt == "f32" else (V / 16 + 16) * 2 * U
     close(got, want, adds * terms + 2 * U * want.abs(), dtype)
+
+
+@pytest.mark.parametrize("how", ["bias", "autocast"])
+def test_z_loss_where_the_logits_are_kept(how):
+    """The z-loss is refused only where the frozen head drops the logits: with a trained bias, and under
+    autocast, it has its gradient."""
+    from test_gpu_distill import model_with_head_norms, teacher_batch
+    from zotitan_b200.losses import distill_xentropy
+    m = model_with_head_norms(seed=30, layers=1).float()
+    for p in m.parameters():
+        p.requires_grad_(False)
+    wq = m.model.layers[0].self_attn.q_norm.weight.requires_grad_(True)
+    batch = teacher_batch(2, 16, 10, seed=31)
+    params = [wq]
+    if how == "bias":
+        head = torch.nn.Linear(256, 1000, device="cuda")
+        head.weight.data.copy_(m.lm_head.weight)
+        head.weight.requires_grad_(False)
+        m.lm_head = head
+        params.append(head.bias)
+    import contextlib
+    with torch.autocast("cuda", torch.bfloat16) if how == "autocast" else contextlib.nullcontext():
+        loss, z, _ = distill_xentropy(m, batch, 1.0, z_loss_weight=1e-2)
+        grads = torch.autograd.grad(loss + z, params)
+        alone = torch.autograd.grad(distill_xentropy(m, batch, 1.0)[0], params)
+    assert all(torch.isfinite(t).all() for t in grads) and not torch.equal(grads[-1], alone[-1])
+    frozen = m.lm_head
+    if how == "bias":
+        frozen.bias.requires_grad_(False)
+    with pytest.raises(NotImplementedError):
+        distill_xentropy(m, batch, 1.0, z_loss_weight=1e-2)

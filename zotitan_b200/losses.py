@@ -153,18 +153,24 @@ class _FrozenHeadDistill(torch.autograd.Function):
         return torch.mul(dx, g[:, None], out=torch.empty_like(dx, dtype=dtype)), None, None, None, None, None, None
 
 
+def _drops_logits(hidden, weight, bias) -> bool:
+    """Whether head_distill, with gradients, keeps no logits: a head that is not trained, outside autocast."""
+    return (torch.is_grad_enabled() and hidden.requires_grad and not torch.is_autocast_enabled("cuda")
+            and not weight.requires_grad and (bias is None or not bias.requires_grad))
+
+
 def head_distill(hidden: torch.Tensor, top_idx: torch.Tensor, top_logits: torch.Tensor, weight: torch.Tensor, bias=None,
                  temperature: float = 1.0, chunk_rows: int = CHUNK_ROWS):
     """Per-row (loss, lse) of hidden rows [R, d] through the head against the teacher's lists
     [R, top] (kernels.distill_rows): without gradients the fused kernel (zt_linear_distill)
     when it takes the operands, which does not round the logits, else a chunk of rows at a
     time through the GEMM and zt_distill_rows. Differentiable in hidden, and in the head
-    where that requires grad (then the whole logits are kept, as the backward needs them);
-    lse is differentiable only in that last form."""
+    where that requires grad (then, and under autocast, the whole logits are kept, as the
+    backward needs them); lse is differentiable only in that last form."""
     train_head = weight.requires_grad or (bias is not None and bias.requires_grad)
     if torch.is_grad_enabled() and (train_head or torch.is_autocast_enabled("cuda")):
         return K.distill_rows(F.linear(hidden, weight, bias), top_idx, top_logits, temperature)
-    if torch.is_grad_enabled() and hidden.requires_grad:
+    if _drops_logits(hidden, weight, bias):
         return _FrozenHeadDistill.apply(hidden, weight, bias, top_idx, top_logits, temperature, chunk_rows)
     if bias is None and K.linear_xent_supported(hidden, weight):
         return K.linear_distill(hidden, weight, top_idx, top_logits, temperature)
@@ -195,9 +201,10 @@ def distill_xentropy(model, batch, temperature: float = 1.0, z_loss_weight: floa
         raise ValueError("teacher_idx and teacher_logits must be [batch, positions, top]")
     hidden = hidden.reshape(-1, hidden.shape[-1])
     idx, val = idx.reshape(-1, idx.shape[-1]), val.reshape(-1, val.shape[-1])
-    if z_loss_weight != 0.0 and torch.is_grad_enabled() and hidden.requires_grad and not head.weight.requires_grad:
+    bias = getattr(head, "bias", None)
+    if z_loss_weight != 0.0 and _drops_logits(hidden, head.weight, bias):
         raise NotImplementedError("the z-loss has no gradient through a frozen head: use z_loss_weight=0")
-    loss, lse = head_distill(hidden, idx, val, head.weight, getattr(head, "bias", None), temperature)
+    loss, lse = head_distill(hidden, idx, val, head.weight, bias, temperature)
     n = ((idx >= 0) & (val != -float("inf"))).any(-1).sum().clamp_min(1)
     value = loss.sum() / n
     return value, None if z_loss_weight == 0.0 else z_loss_weight * lse.square().sum() / n, None
