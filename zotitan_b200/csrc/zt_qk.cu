@@ -796,7 +796,7 @@ int check_args(const zt_qk_args* a, bool backward, const char* who) {
     return zt::set_error(ZT_ERR_INVALID, w + ": weights and tables must have the heads' dtype or fp32");
   if (a->table_batch != 0 && a->table_batch != 1) return zt::set_error(ZT_ERR_INVALID, w + ": table_batch must be 0 or 1");
   if (!(a->eps >= 0.f) || isinf(a->eps)) return zt::set_error(ZT_ERR_INVALID, w + ": eps must be finite and not negative");
-  if (a->seq > 0 && a->batch > (int64_t)(INT32_MAX / 64) / a->seq)
+  if (a->seq > 0 && a->batch > ((int64_t)1 << 25) / a->seq)
     return zt::set_error(ZT_ERR_LIMIT, w + ": more than 2^25 positions");
   if (a->q_heads > 65535 || a->k_heads > 65535) return zt::set_error(ZT_ERR_LIMIT, w + ": more than 65535 heads");
   if (a->batch * a->seq == 0 && !backward) return ZT_OK;
