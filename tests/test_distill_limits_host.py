@@ -14,3 +14,17 @@ def test_positions_up_to_the_documented_limit(lib, batch, seq, fits):  # noqa: F
     for fn in (lib.zt_qk_norm_rope, lib.zt_qk_norm_rope_backward):
         assert fn(ctypes.byref(qk_args(batch=batch, seq=seq, q=None)), None) == (L.ZT_ERR_INVALID if fits else L.ZT_ERR_LIMIT)
         assert (b"null pointer" if fits else b"2^25") in lib.zt_last_error()
+
+
+@pytest.mark.parametrize("version", [11, 3])
+def test_library_of_another_build(tmp_path, monkeypatch, version):
+    """A library without some of the entry points, or of another version, says so when it is loaded."""
+    import subprocess
+    src, so = tmp_path / "old.c", tmp_path / "old.so"
+    src.write_text(f"int zt_abi_version(void) {{ return {version}; }}\nconst char* zt_last_error(void) {{ return \"\"; }}\n")
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)])
+    monkeypatch.setattr(L, "_lib", None)
+    monkeypatch.setattr(L, "LIB_PATH", str(so))
+    with pytest.raises(L.ZtError, match="zt_distill_rows" if version == L.ABI_VERSION else "ABI version 3"):
+        L.load()
+    assert L._lib is None

@@ -200,9 +200,15 @@ def load():
                       "(the zeroth-order kernels have no CPU fallback)")
     lib = ctypes.CDLL(LIB_PATH)
     P, I32, I64, U32, U64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint64
+    lib.zt_abi_version.restype = ctypes.c_int
+    if lib.zt_abi_version() != ABI_VERSION:
+        raise ZtError(f"{LIB_PATH}: ABI version {lib.zt_abi_version()} != {ABI_VERSION}")
+    missing = [name for name in EXPORTS if not hasattr(lib, name)]   # entry points may be added within a version
+    if missing:
+        raise ZtError(f"{LIB_PATH} is older than this package (no {', '.join(missing)}): build it with "
+                      "`python -m zotitan_b200.build`")
     lib.zt_last_error.restype = ctypes.c_char_p
     lib.zt_last_error.argtypes = []
-    lib.zt_abi_version.restype = ctypes.c_int
     lib.zt_param_key.restype = U32
     lib.zt_param_key.argtypes = [U64, U32, U32]
     for name, args in [("zt_philox_words", [U32, P, I64, P, P]), ("zt_randn", [U32, I64, I64, P, P]),
@@ -292,8 +298,6 @@ def load():
     lib.zt_qk_norm_rope_workspace_bytes.argtypes = [I32]
     lib.zt_plan_workspace_bytes.restype = ctypes.c_size_t
     lib.zt_plan_workspace_bytes.argtypes = [I32]
-    if lib.zt_abi_version() != ABI_VERSION:
-        raise ZtError(f"{LIB_PATH}: ABI version {lib.zt_abi_version()} != {ABI_VERSION}")
     _lib = lib
     return lib
 
