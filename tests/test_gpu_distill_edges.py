@@ -157,3 +157,84 @@ def test_z_loss_where_the_logits_are_kept(how):
         frozen.bias.requires_grad_(False)
     with pytest.raises(NotImplementedError):
         distill_xentropy(m, batch, 1.0, z_loss_weight=1e-2)
+
+
+# an odd and an even number of accumulators a tile, whole and partial last ones, several row tiles
+@pytest.mark.parametrize("R,V,k,top,T", [(300, 1537, 1088, 40, 1.0), (300, 1537, 2112, 64, 2.0), (600, 4097, 3136, 16, 1.0),
+                                         (257, 700, 2048, 256, 0.7)])
+def test_head_of_several_accumulators(R, V, k, top, T):
+    """Tolerances as in test_gpu_distill.test_linear."""
+    from zotitan_b200 import kernels as K
+    x, w, idx, val = operands(R, V, k, top, seed=24)
+    loss, lse = K.linear_distill(x, w, idx, val, T)
+    assert K.linear_distill_take_error() == 0
+    e = Exact(x.double() @ w.double().t(), idx, val, T)
+    ez = (k / 16 + 16) * 2 * U * (x.double().abs() @ w.double().abs().t()).amax(1)
+    close(loss, e.loss, e.tol_loss + 2 * T * ez, torch.float32)
+    close(lse, e.lse, e.tol_lse + ez / T, torch.float32)
+
+
+def test_pieces_of_k_are_added_in_fp32():
+    """A logit of K 8192 is the sum of its eight pieces of 1024, rounded to nearest as they are added:
+    with a vocabulary of one, lse is the logit. Each lse is rounded four times (the base's product with
+    log2 e, that with ln 2, both constants: 4 u of it) and seven adds round once: (4 + 4 + 7) u of the
+    logit, u = 2^-24. One accumulator for all of K would truncate at each of its 512 steps, a third of
+    u of the logit every time, where the pieces lose an eighth of that: 150 u apart."""
+    from zotitan_b200 import kernels as K
+    g = torch.Generator(device="cuda").manual_seed(25)
+    R, k = 300, 8192
+    x = (torch.rand(R, k, device="cuda", generator=g) + 0.5).bfloat16()
+    w = (torch.rand(1, k, device="cuda", generator=g) + 0.5).bfloat16()
+    idx, val = torch.zeros(R, 1, dtype=torch.int64, device="cuda"), torch.zeros(R, 1, device="cuda")
+    whole = K.linear_distill(x, w, idx, val)[1].double()
+    pieces = sum(K.linear_distill(x[:, j:j + 1024].contiguous(), w[:, j:j + 1024].contiguous(), idx, val)[1].double()
+                 for j in range(0, k, 1024))
+    assert float(((whole - pieces).abs() / pieces).max()) <= 15 * U
+
+
+def c_args(z, idx, val, T, grad, weight=None, weight_lse=None, loss=None, lse=None, stats=None):
+    from zotitan_b200 import _lib as L
+    a = L.ZtDistillArgs()
+    a.logits, a.grad, a.top_idx, a.top_logits = z.data_ptr(), grad.data_ptr(), idx.data_ptr(), val.data_ptr()
+    for name, t in (("weight", weight), ("weight_lse", weight_lse), ("loss", loss), ("lse", lse), ("stats", stats)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    a.rows, a.vocab, a.ld, a.ld_grad = *z.shape, z.stride(0), grad.stride(0)
+    a.dtype = {torch.float32: L.ZT_F32, torch.bfloat16: L.ZT_BF16, torch.float16: L.ZT_F16}[z.dtype]
+    a.top, a.idx_bits, a.top_dtype, a.temperature = idx.shape[1], 64, L.ZT_F32, T
+    return a
+
+
+# a warp a row, a CTA a row (narrow and wide), a cluster of CTAs a row
+@pytest.mark.parametrize("dt,rows,vocab,shift", [("bf16", 1500, 1003, 1), ("f32", 700, 8192, 0), ("f16", 320, 70001, 1), ("bf16", 9, 50257, 3)])
+def test_c_entry_points_beyond_the_wrappers(dt, rows, vocab, shift):
+    """zt_distill_rows_grad with a gradient of lse and with stats for a later backward, and
+    zt_distill_rows_backward in place."""
+    from zotitan_b200 import _lib as L
+    lib, dtype, T = L.load(), DTYPES[dt], 2.0
+    z, idx, val = make(rows, vocab, 33, dtype, T, ld=vocab + 5, seed=28, shift=shift)
+    idx, val = idx.contiguous(), val.contiguous()
+    gen = torch.Generator(device="cuda").manual_seed(29)
+    g, gl = (torch.rand(rows, device="cuda", generator=gen) * 64 + 0.5 for _ in range(2))
+    stream = torch.cuda.current_stream().cuda_stream
+    e = Exact(z, idx, val, T)
+    want, tol = e.grad(g, gl)
+    loss, lse = (torch.empty(rows, device="cuda") for _ in range(2))
+    stats = torch.empty(rows, 2, device="cuda")
+    one = torch.empty_like(z)
+    assert lib.zt_distill_rows_grad(ctypes.byref(c_args(z, idx, val, T, one, g, gl, loss, lse, stats)), stream) == L.ZT_OK
+    close(one, want, tol, dtype)
+    close(loss, e.loss, e.tol_loss, torch.float32)
+    close(lse, e.lse, e.tol_lse, torch.float32)
+    two = torch.empty_like(z)
+    assert lib.zt_distill_rows_backward(ctypes.byref(c_args(z, idx, val, T, two, g, gl, stats=stats)), stream) == L.ZT_OK
+    close(two, want, tol, dtype)
+    gap = torch.as_strided(z, (rows - 1, 5), (z.stride(0), 1), z.storage_offset() + vocab).clone()
+    assert lib.zt_distill_rows_backward(ctypes.byref(c_args(z, idx, val, T, z, g, gl, stats=stats)), stream) == L.ZT_OK
+    close(z, want, tol, dtype)
+    assert torch.equal(torch.as_strided(z, (rows - 1, 5), (z.stride(0), 1), z.storage_offset() + vocab), gap)   # behind each row
+    # a gradient of lse alone
+    z2, _, _ = make(rows, vocab, 33, dtype, T, ld=vocab + 5, seed=28, shift=shift)
+    want, tol = e.grad(None, gl)
+    assert lib.zt_distill_rows_backward(ctypes.byref(c_args(z2, idx, val, T, two, None, gl, stats=stats)), stream) == L.ZT_OK
+    close(two, want, tol, dtype)
