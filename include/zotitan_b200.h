@@ -585,7 +585,8 @@ ZT_API size_t zt_linear_xent_workspace_bytes(int64_t rows, int64_t vocab, int64_
 ZT_API int zt_linear_xent(const zt_lce_args* args, void* stream);
 
 /* Reads and clears the fused scorer's device error flag (nonzero: a bounded wait inside
- * the GEMM expired; its outputs are then incomplete). Synchronises with the device. */
+ * the GEMM expired; loss and lse of the rows it did not finish are then NaN and correct 0, ignored
+ * rows aside). Synchronises with the device. */
 ZT_API int zt_linear_xent_take_error(int32_t* code);
 
 /* ---- distillation from a teacher's top logits --------------------------------------- */

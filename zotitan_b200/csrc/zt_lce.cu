@@ -17,7 +17,8 @@
 // the item they write these four numbers per row to a small partials buffer.
 // Kernel 2 (lce_combine_kernel) merges each row's splits in vocabulary order.
 // Every mbarrier wait is bounded; on expiry the kernel records an error
-// (zt_linear_xent_take_error), drains its own copies and MMAs and frees its tensor memory.
+// (zt_linear_xent_take_error), drains its own copies and MMAs, frees its tensor memory and leaves
+// NaN for every sum that it did not finish.
 #include <math.h>
 
 #include "zt_tc.cuh"
@@ -49,6 +50,10 @@ struct LceParams {
   int32_t stall_loads;    // test hook: the loader issues no copies
   long long wait_cycles;  // bound of every wait
 };
+
+// The part of a row that an expired wait left undone: its loss and lse become NaN, and no column its
+// maximum.
+__device__ __forceinline__ float4 unfinished() { return make_float4(INFINITY, NAN, NAN, __int_as_float(-1)); }
 
 __device__ __forceinline__ void item_range(const LceParams& P, int item, int& mt, int& split, int& nt0, int& nt1) {
   split = item / P.m_tiles;
@@ -170,10 +175,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t leader_acce0 = peer_addr(&acce[0], 0), leader_acce1 = peer_addr(&acce[1], 0);
     uint32_t tcount = 0;
     bool ok = true;
-    for (int item = cid; ok && item < n_items; item += ncl) {
+    for (int item = cid; item < n_items; item += ncl) {
       int mt, split, nt0, nt1;
       item_range(P, item, mt, split, nt0, nt1);
       const int row = mt * (int)kTile + (int)rank * (int)kHalfRows + row_local;
+      if (!ok) {   // a wait has expired: what is left of the queue is not a number
+        if (row < P.rows) P.partials[(size_t)split * P.rows_pad + row] = unfinished();
+        continue;
+      }
       const int64_t t = row < P.rows ? __ldg(P.targets + row) : -1;
       float m = -INFINITY, s = 0.f, tgt = __int_as_float(0x7fc00000);  // NaN: target not in this split
       int amax = -1;
@@ -231,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(b ? leader_acce1 : leader_acce0);  // accumulator b may be overwritten
       }
-      if (ok && row < P.rows) P.partials[(size_t)split * P.rows_pad + row] = make_float4(m, s, tgt, __int_as_float(amax));
+      if (row < P.rows) P.partials[(size_t)split * P.rows_pad + row] = ok ? make_float4(m, s, tgt, __int_as_float(amax)) : unfinished();
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
