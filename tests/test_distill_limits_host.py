@@ -114,3 +114,19 @@ def test_linear_distill_arguments_as_the_header_lays_them_out(recorder, monkeypa
     assert got == dict(x=ptr(x), w=ptr(w), top_idx=ptr(idx), top_logits=ptr(val), loss=ptr(loss), lse=ptr(lse), workspace_bytes=4096, rows=6,
                        vocab=17, k=64, top=3, idx_bits=64, top_dtype=L.ZT_F32, temperature=0.5, test_stall_loads=1, reserved=0,
                        test_wait_cycles=12345)
+
+
+@pytest.mark.parametrize("dt", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("vocab,ld,shift", [(1000, 1000, 0), (1000, 1001, 1), (1003, 1003, 3), (1003, 50 * 1003, 7), (17, 24, 5), (1, 9, 2)])
+def test_gradient_room_is_aligned_as_the_logits_are(dt, vocab, ld, shift):
+    """Every row of the gradient starts at the 16-byte phase of its row of logits, within a row more of room."""
+    import torch
+
+    from zotitan_b200 import kernels as K
+    dtype = getattr(torch, dt)
+    x = torch.zeros(4 * ld + shift, dtype=dtype)[shift:].view(4, ld)[:, :vocab]
+    g = K._grad_of(x)
+    assert g.shape == x.shape and g.dtype == dtype and g.stride(1) == 1 and g.stride(0) >= vocab
+    for r in range(4):
+        assert g[r].data_ptr() % 16 == x[r].data_ptr() % 16
+    assert g.untyped_storage().nbytes() <= 4 * (vocab + 8) * x.element_size() + 16

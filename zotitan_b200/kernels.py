@@ -1175,10 +1175,15 @@ def _ld(t: torch.Tensor) -> int:
 
 
 def _grad_of(x: torch.Tensor) -> torch.Tensor:
-    """Room for the gradient of x: rows aligned as x's are, with less than a row between them (x may
-    be one position of every sequence, whose row stride is a whole sequence)."""
-    vocab = x.shape[1]
-    return x.new_empty_strided(x.shape, (vocab + (_ld(x) - vocab) % 8, 1))   # 8 elements: 16 or 32 bytes
+    """Room for the gradient of x: rows aligned as x's are (x may start anywhere, as logits[:, 1:] does),
+    with less than a row between them (x may be one position of every sequence, whose row stride
+    is a whole sequence)."""
+    rows, vocab = x.shape
+    ld = vocab + (_ld(x) - vocab) % 8   # 8 elements: 16 or 32 bytes
+    phase = x.data_ptr() % 16 // x.element_size()
+    if phase == 0 or rows == 0:
+        return x.new_empty_strided((rows, vocab), (ld, 1))
+    return x.new_empty(phase + (rows - 1) * ld + vocab).as_strided((rows, vocab), (ld, 1), phase)
 
 
 def _distill_call(entry, x, top_idx, top_logits, temperature, grad=None, weight=None, weight_lse=None, loss=0, lse=0, stats=0):
