@@ -23,10 +23,12 @@ using zt::tc::cluster_rank;
 using zt::tc::cluster_sync_all;
 using zt::tc::peer_addr;
 
-// Threads that stream a row, beside the list's warp, and the CTAs of an SM. A thread's step is two
-// vectors in the forward and four elsewhere. The forward lives on warps: of 4096 x 128256 bf16 it
-// takes 180 us with six CTAs of two vectors, 184 with four of four, 199 to 226 where
-// a thread also loads its next step ahead (its registers cost warps).
+// Threads that stream a row, beside the list's warp, and the CTAs of an SM that the compiler is asked
+// for. A thread's step is two vectors in the forward and four elsewhere. The forward lives on warps: of
+// 4096 x 128256 bf16 it takes 180 us with six CTAs of two vectors, 184 with four of four, 199 to
+// 226 where a thread also loads its next step ahead (its registers cost warps). Asked for six it
+// takes 32 registers (the 16-bit ones spill six of them), with which seven are resident; the rules below
+// count six.
 constexpr int kSumThreads = 256, kSumCtas = 6, kSumStep = 2;
 // The backward, and loss and gradient at once: rows of up to kMidRow bytes go to CTAs half as wide,
 // twice as many (4000 x 32000 bf16, 64 KB: 117 us so, 152 with the wide ones; 2048 x 100000, 200 KB:
@@ -523,7 +525,8 @@ __global__ void __launch_bounds__(S + 32, CTAS) distill_backward_kernel(const __
 
 // Loss and gradient at once: the sum reads the row from memory, the gradient reads it again from
 // L2. (Held in the shared memory of a cluster of four instead, the row's loads, sums and
-// stores took turns: 2048 x 128256 bf16 257 us, so 213.)
+// stores took turns: 2048 x 128256 bf16 257 us, so 223 with the same inner loop; 213 with the
+// unpredicated steps that came later, with which the other form was not measured.)
 template <int DT, int S, int CTAS>
 __global__ void __launch_bounds__(S + 32, CTAS) distill_grad_kernel(const __grid_constant__ RowsParams P) {
   using T = typename El<DT>::T;

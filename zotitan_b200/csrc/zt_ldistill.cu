@@ -14,7 +14,9 @@
 //    so that the pairs in flight share W tiles in L2. The tensor cores truncate as they
 //    accumulate: over a K of 2048 that alone puts the loss 1.8e-6 off, over 4096 3.6e-6. So an
 //    accumulator takes 1024 of K, and the epilogue threads add these up in registers, rounding
-//    to nearest: 0.9e-6 at any K, for 1.5% of the time (512 of K: 0.4e-6 for 6%).
+//    to nearest: 0.9e-6 at any K, for 1.5% of the time. Smaller pieces cost more than they give here:
+//    512 of K halves the error again for 6 to 9% (8192 x 128256 x 2048 3.2 -> 3.4 ms, 2048 x 32000 x 2048
+//    225 -> 249 us), 256 quarters it for 38%. The bf16 operands are up to 2^-8 = 4e-3 of themselves off.
 //    An epilogue thread owns half an accumulator row, 128 columns. It also follows the part of
 //    its row's list that lies in its columns through the tiles: where one of a warp's rows has
 //    a listed token among 16 columns, its threads put theirs into shared memory, each for itself,
