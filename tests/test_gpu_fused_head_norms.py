@@ -306,3 +306,16 @@ def test_replaced_forwards_are_called():
                         out.append(PARTS[part](model, x, pe).float())
                 scale = float(out[0].square().mean().sqrt())
                 assert float((out[0] - out[1]).square().mean().sqrt()) <= 0.02 * scale, (part, name, before)
+
+
+def test_compiled_llama():
+    """A fused Llama under torch.compile: its modules' own code, as compiled without fuse_llama."""
+    from zotitan_b200.llama_fused import unfuse_llama
+    m = llama_attention()
+    ids = torch.arange(40, device="cuda").view(2, 20) % 100
+    torch._dynamo.reset()
+    with torch.inference_mode():
+        got = torch.compile(lambda i: m(input_ids=i, use_cache=False).logits, backend="eager")(ids)
+        unfuse_llama(m)
+        assert torch.equal(got, m(input_ids=ids, use_cache=False).logits)
+    torch._dynamo.reset()

@@ -33,7 +33,7 @@ Each other fused forward defers to the module's own forward when gradients are e
 the activations are not bf16 on a CUDA device, the layout does not fit (head_dim not a
 multiple of 16, per-sequence position ids), or the MLP's activation is not SiLU. All of them
 do where torch itself has to follow the operations: under forward-mode derivatives, in a trace,
-inside torch.func's transforms and, those of decoders with head norms, under torch.compile.
+inside torch.func's transforms and under torch.compile.
 `unfuse_llama(model)` restores the original forwards.
 """
 from __future__ import annotations
@@ -66,18 +66,15 @@ def assume_causal():
         _ASSUME_CAUSAL = prev
 
 
-def _torch_must_see(m: nn.Module) -> bool:
+def _torch_must_see() -> bool:
     """Calls whose operations torch itself follows, which a kernel launch hides from it: forward-mode
-    derivatives (torch.no_grad leaves them on), traces, torch.func's transforms. And torch.compile for
-    decoders with head norms; fused Llama forwards break its graph and run as they do outside of it."""
-    if torch.compiler.is_compiling():
-        return type(m).__name__.startswith("Qwen3")
-    return (forward_ad._current_level >= 0 or torch._C._is_tracing()
+    derivatives (torch.no_grad leaves them on), traces, torch.func's transforms, torch.compile."""
+    return (torch.compiler.is_compiling() or forward_ad._current_level >= 0 or torch._C._is_tracing()
             or torch._C._functorch.peek_interpreter_stack() is not None)
 
 
-def _fast(m: nn.Module, x: torch.Tensor) -> bool:
-    return (not torch.is_grad_enabled()) and x.is_cuda and x.dtype == torch.bfloat16 and not _torch_must_see(m)
+def _fast(x: torch.Tensor) -> bool:
+    return (not torch.is_grad_enabled()) and x.is_cuda and x.dtype == torch.bfloat16 and not _torch_must_see()
 
 
 def _unhooked(m: nn.Module) -> bool:
@@ -103,7 +100,7 @@ def _ours(m: nn.Module) -> bool:
 
 def _rmsnorm_forward(self, hidden_states):
     w = self.weight
-    if (not _fast(self, hidden_states) or w.dtype != torch.bfloat16 or hidden_states.shape[-1] % 8
+    if (not _fast(hidden_states) or w.dtype != torch.bfloat16 or hidden_states.shape[-1] % 8
             or not hidden_states.is_contiguous()):
         return self._zt_orig_forward(hidden_states)
     return K.rmsnorm(hidden_states, w.detach(), self.variance_epsilon)
@@ -113,7 +110,7 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
                        **kwargs):
     cos, sin = position_embeddings if position_embeddings is not None else (None, None)
     hd = self.head_dim
-    if (not _fast(self, hidden_states) or cos is None or cos.shape[0] != 1 or hd % 16 or cos.dtype != torch.bfloat16
+    if (not _fast(hidden_states) or cos is None or cos.shape[0] != 1 or hd % 16 or cos.dtype != torch.bfloat16
             or hidden_states.dim() != 3):
         return self._zt_orig_forward(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
     from transformers.models.llama.modeling_llama import ALL_ATTENTION_FUNCTIONS, eager_attention_forward
@@ -148,7 +145,7 @@ def _qk_norm_attention_forward(self, hidden_states, position_embeddings=None, at
     cos, sin = position_embeddings if position_embeddings is not None else (None, None)
     hd = self.head_dim
     dt = hidden_states.dtype
-    if _torch_must_see(self) or not _plain_norm(self.q_norm, hd) or not _plain_norm(self.k_norm, hd):
+    if _torch_must_see() or not _plain_norm(self.q_norm, hd) or not _plain_norm(self.k_norm, hd):
         return self._zt_orig_forward(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
     wq, wk = self.q_norm.weight, self.k_norm.weight
     eps = self.q_norm.variance_epsilon
@@ -193,7 +190,7 @@ def _plain_linear(m, k: int) -> bool:
 
 
 def _mlp_forward(self, x):
-    if not _fast(self, x) or not is_silu(self.act_fn) or not _untouched(self.act_fn):
+    if not _fast(x) or not is_silu(self.act_fn) or not _untouched(self.act_fn):
         return self._zt_orig_forward(x)
     k = x.shape[-1]
     rows = x.numel() // k
